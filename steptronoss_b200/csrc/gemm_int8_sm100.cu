@@ -1,0 +1,515 @@
+// 8-bit integer GEMM for sm_100a with one scale per token and one per output channel:
+//
+//     Y[m, n] = sx[m] * sw[n] * sum_k Xq[m, k] * Wq[n, k]          Xq [M, K], Wq [N, K] int8, sums in int32, Y bf16/fp32
+//
+// tcgen05.mma.kind::i8 accumulates in int32, so the product is exact and independent of the order of its sums; K is at
+// most 131071 (2^31 / 128^2).  The sum is converted to fp32 once, multiplied by the two scales and rounded to Y's type.
+//
+// The weights are the A operand (128 channels of the tile are the 128 TMEM lanes) and the tokens the B operand (TMEM
+// columns), whatever their number: a decode step of a few tokens then takes a 16-, 32- or 64-column tile instead of
+// a mostly empty 128-row one, and a warp that reads one column writes 32 neighbouring channels of one token.
+//
+//   gemm_int8_kernel        many tokens: persistent, 128 x 256 tiles, accumulators double-buffered in TMEM
+//   gemm_int8_split_kernel  few tokens: one tile per cluster, K cut over the CTAs of the cluster so that the weights
+//                           stream through all SMs; partial sums meet in distributed shared memory
+#include "common.cuh"
+
+namespace stb {
+
+constexpr int kI8BlockN = 128;      // channels per tile
+constexpr int kI8BlockK = 128;      // one 128-byte swizzle span
+constexpr int kI8WTile = kI8BlockN * kI8BlockK;
+constexpr int kI8Threads = 192;     // producer, MMA issuer, four epilogue warps
+
+struct Int8GemmParams {
+  int M, N, K;
+  long long ldy;
+  const float* sx;
+  const float* sw;
+  void* Y;
+  int* status;
+  int tma_out;                      // bf16 output that a tensor map describes
+};
+
+// kind::i8: int32 accumulators (D format 2), signed 8-bit A and B (format 1), both K-major
+__host__ __device__ constexpr uint32_t umma_idesc_s8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// 4 steps of K = 32 over one 128-byte swizzle span; `accumulate` applies to the first step only.
+__device__ __forceinline__ void umma4_s8(uint32_t d, uint64_t a0, uint64_t b0, uint32_t idesc, uint32_t accumulate) {
+  const uint64_t a1 = umma_desc_advance(a0, 32), a2 = umma_desc_advance(a0, 64), a3 = umma_desc_advance(a0, 96);
+  const uint64_t b1 = umma_desc_advance(b0, 32), b2 = umma_desc_advance(b0, 64), b3 = umma_desc_advance(b0, 96);
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %10, 0;\n\t"
+      "setp.eq.b32 q, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %5, %9, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %2, %6, %9, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %3, %7, %9, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %4, %8, %9, q;\n\t}"
+      ::"r"(d), "l"(a0), "l"(a1), "l"(a2), "l"(a3), "l"(b0), "l"(b1), "l"(b2), "l"(b3), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 16 consecutive columns: thread t of the warp receives row (lane base + t).
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------- many tokens
+template <int BM>                   // tokens per tile
+struct Int8Smem {
+  static constexpr int kStages = BM == 256 ? 4 : 6;
+  static constexpr int kXTile = BM * kI8BlockK;
+  static constexpr int kStageBytes = kI8WTile + kXTile;
+  static constexpr int kStoreBytes = 4 * 2 * 4096;    // per epilogue warp: two tiles of 64 tokens x 32 channels bf16
+  static constexpr int kTotal = kStages * kStageBytes + kStoreBytes + 256 + 1024;
+};
+
+// Tiles are walked in bands of kBand channel tiles so that the CTAs of a wave share weights and tokens in L2.
+__device__ __forceinline__ void int8_tile(int tile, int num_n, int num_m, int& n_tile, int& m_tile) {
+  constexpr int kBand = 16;
+  const int band = tile / (kBand * num_m);
+  const int first = band * kBand;
+  const int rows = min(num_n - first, kBand);
+  const int r = tile - band * kBand * num_m;
+  n_tile = first + r % rows;
+  m_tile = r / rows;
+}
+
+template <typename TY>
+__device__ __forceinline__ void store_y(TY* p, float v);
+template <> __device__ __forceinline__ void store_y<float>(float* p, float v) { *p = v; }
+template <> __device__ __forceinline__ void store_y<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <int BM, typename TY>
+__global__ void __launch_bounds__(kI8Threads, 1)
+gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                 const __grid_constant__ CUtensorMap tmap_y, const Int8GemmParams p) {
+  using S = Int8Smem<BM>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* store_stage = smem + kStages * S::kStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(store_stage + S::kStoreBytes);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* tmem_full = empty_bar + kStages;
+  uint64_t* tmem_empty = tmem_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_n = (p.N + kI8BlockN - 1) / kI8BlockN;
+  const int num_m = (p.M + BM - 1) / BM;
+  const int num_tiles = num_n * num_m;
+  const int k_blocks = (p.K + kI8BlockK - 1) / kI8BlockK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tmem_full[a], 1);
+      mbar_init(&tmem_empty[a], 4);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 2 * BM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int tile = blockIdx.x; tile < num_tiles && !*abort_flag; tile += gridDim.x) {
+        int n_tile, m_tile;
+        int8_tile(tile, num_n, num_m, n_tile, m_tile);
+        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&empty_bar[s], ((it / kStages) & 1) ^ 1)) {
+            report_error(p.status, kErrProducerWait);
+            *abort_flag = 1;
+            break;
+          }
+          uint8_t* sw = smem + s * S::kStageBytes;
+          mbar_arrive_expect_tx(&full_bar[s], S::kStageBytes);
+          tma_load_2d(sw, &tmap_w, &full_bar[s], kb * kI8BlockK, n_tile * kI8BlockN);
+          tma_load_2d(sw + kI8WTile, &tmap_x, &full_bar[s], kb * kI8BlockK, m_tile * BM);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_s8(kI8BlockN, BM);
+      uint32_t it = 0, local = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < num_tiles && ok && !*abort_flag; tile += gridDim.x, ++local) {
+        const int acc = local & 1;
+        ok = mbar_wait(&tmem_empty[acc], ((local >> 1) & 1) ^ 1);
+        if (!ok) { report_error(p.status, kErrMmaWaitTmem); break; }
+        tc_fence_after();
+        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+          const int s = it % kStages;
+          ok = mbar_wait(&full_bar[s], (it / kStages) & 1);
+          if (!ok) { report_error(p.status, kErrMmaWaitFull); break; }
+          tc_fence_after();
+          const uint32_t sw = smem_u32(smem + s * S::kStageBytes);
+          umma4_s8(tmem_base + acc * BM, umma_smem_desc(sw, 16, 1024), umma_smem_desc(sw + kI8WTile, 16, 1024), idesc,
+                   kb > 0 ? 1u : 0u);
+          umma_commit(&empty_bar[s]);
+        }
+        if (!ok) break;
+        umma_commit(&tmem_full[acc]);
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    const int quarter = warp & 3;
+    uint8_t* my_stage = store_stage + (warp - 2) * 8192;
+    uint32_t local = 0, stores = 0;
+    for (int tile = blockIdx.x; tile < num_tiles && !*abort_flag; tile += gridDim.x, ++local) {
+      int n_tile, m_tile;
+      int8_tile(tile, num_n, num_m, n_tile, m_tile);
+      const int acc = local & 1;
+      const int n = n_tile * kI8BlockN + quarter * 32 + lane, m0 = m_tile * BM;
+      const float sw = n < p.N ? p.sw[n] : 0.f;
+      bool ok = mbar_wait(&tmem_full[acc], (local >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) { report_error(p.status, kErrEpilogueWait); *abort_flag = 1; break; }
+      tc_fence_after();
+      const int cols = min(BM, p.M - m0);
+#pragma unroll 1
+      for (int c = 0; c < cols; c += 32) {
+        const float sx = c + lane < cols ? p.sx[m0 + c + lane] : 0.f;
+        uint32_t v[32];
+        tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BM + c, v);
+        tmem_wait_ld();
+        if (p.tma_out) {
+          uint8_t* buf = my_stage + (stores & 1) * 4096;
+          if ((c & 32) == 0 && stores >= 2) {
+            if (lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+          }
+          __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(buf) + (c & 32) * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            out[j * 32] = __float2bfloat16_rn(static_cast<float>(static_cast<int>(v[j])) * __shfl_sync(0xffffffffu, sx, j) * sw);
+          if ((c & 32) != 0 || c + 32 >= cols) {   // 64 tokens staged, or the last of the tile
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              const int n0 = n_tile * kI8BlockN + quarter * 32;
+              if (n0 < p.N) tma_store_2d(&tmap_y, buf, n0, m0 + (c & ~63));   // rows and channels past the end are clipped
+              tma_store_commit();
+            }
+            ++stores;
+          }
+        } else {
+          TY* y = static_cast<TY*>(p.Y) + static_cast<long long>(m0 + c) * p.ldy + n;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float f = static_cast<float>(static_cast<int>(v[j])) * __shfl_sync(0xffffffffu, sx, j) * sw;
+            if (n < p.N && c + j < cols) store_y<TY>(y + j * p.ldy, f);
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive_warp(&tmem_empty[acc]);
+    }
+    if (lane == 0) tma_store_wait<0>();
+  }
+
+  __syncthreads();
+  if (*abort_flag) drain_delay();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * BM);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- few tokens
+template <int BM>
+struct Int8SplitSmem {
+  static constexpr int kXTile = BM * kI8BlockK;
+  static constexpr int kStageBytes = kI8WTile + kXTile;
+  static constexpr int kPartBytes = kI8BlockN * BM * 4;       // [source CTA][column of this CTA][128 channels] int32
+  static constexpr int kStages = BM <= 32 ? 5 : BM == 64 ? 4 : 4;
+  static constexpr int kTotal = kStages * kStageBytes + kPartBytes + 256 + 1024;
+};
+
+__device__ __forceinline__ uint32_t i8_cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// One output tile (128 channels, BM tokens) per cluster of S CTAs; CTA r takes every k block kb with kb % S == r.
+// After the products, column c of the tile belongs to CTA c % S: every CTA stores its partial sums of that column into
+// that CTA's shared memory, and after one cluster barrier each CTA adds, scales and writes its columns.
+template <int BM, int S, typename TY>
+__global__ void __launch_bounds__(kI8Threads)
+gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                       const Int8GemmParams p) {
+  using L = Int8SplitSmem<BM>;
+  constexpr int kStages = L::kStages;
+  constexpr int kTmemCols = BM < 32 ? 32 : BM;
+  extern __shared__ uint8_t smem_raw[];
+  // the same offset in every CTA of the cluster: the dynamic segment starts at the same address in all of them
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  int* part = reinterpret_cast<int*>(smem + kStages * L::kStageBytes);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kStages * L::kStageBytes + L::kPartBytes);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* done_bar = empty_bar + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = S > 1 ? static_cast<int>(i8_cluster_rank()) : 0;
+  const int num_n = (p.N + kI8BlockN - 1) / kI8BlockN;
+  const int tile = blockIdx.x / S;
+  const int n_tile = tile % num_n, m_tile = tile / num_n;
+  const int m0 = m_tile * BM, cols = min(BM, p.M - m0);
+  const int all_blocks = (p.K + kI8BlockK - 1) / kI8BlockK;
+  const int k_blocks = (all_blocks - rank + S - 1) / S;     // one at least: S is at most half of all_blocks
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if constexpr (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // running
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < k_blocks; ++i) {
+        const int s = i % kStages;
+        if (!mbar_wait(&empty_bar[s], ((i / kStages) & 1) ^ 1)) {
+          report_error(p.status, kErrProducerWait);
+          *abort_flag = 1;
+          break;
+        }
+        const int kb = i * S + rank;
+        uint8_t* sw = smem + s * L::kStageBytes;
+        mbar_arrive_expect_tx(&full_bar[s], L::kStageBytes);
+        tma_load_2d(sw, &tmap_w, &full_bar[s], kb * kI8BlockK, n_tile * kI8BlockN);
+        tma_load_2d(sw + kI8WTile, &tmap_x, &full_bar[s], kb * kI8BlockK, m0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_s8(kI8BlockN, BM);
+      bool ok = true;
+      for (int i = 0; i < k_blocks; ++i) {
+        const int s = i % kStages;
+        ok = mbar_wait(&full_bar[s], (i / kStages) & 1);
+        if (!ok) { report_error(p.status, kErrMmaWaitFull); *abort_flag = 1; break; }
+        tc_fence_after();
+        const uint32_t sw = smem_u32(smem + s * L::kStageBytes);
+        umma4_s8(tmem_base, umma_smem_desc(sw, 16, 1024), umma_smem_desc(sw + kI8WTile, 16, 1024), idesc, i > 0 ? 1u : 0u);
+        umma_commit(&empty_bar[s]);
+      }
+      umma_commit(done_bar);
+    }
+    __syncwarp();
+  }
+  const int quarter = warp & 3;
+  const int row = quarter * 32 + lane;
+  bool ok = true;
+  if (warp >= 2) {
+    ok = mbar_wait(done_bar, 0);
+    ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
+    if (!ok) report_error(p.status, kErrEpilogueWait);
+    tc_fence_after();
+  }
+  if constexpr (S > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  // columns of the tile in groups of 16; with S > 1 each goes to the CTA that owns it
+  const int n = n_tile * kI8BlockN + row;
+  const float swn = warp >= 2 && n < p.N ? p.sw[n] : 0.f;
+  if (warp >= 2 && ok) {
+    for (int c = 0; c < cols; c += 16) {
+      uint32_t v[16];
+      tmem_ld_32x16(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (c + j >= cols) continue;
+        if constexpr (S > 1) {
+          const int owner = (c + j) % S, slot = (c + j) / S;
+          uint32_t addr;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                       : "=r"(addr) : "r"(smem_u32(part + (rank * (BM / S) + slot) * kI8BlockN + row)), "r"(owner));
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v[j]) : "memory");
+        } else if (n < p.N) {
+          const float f = static_cast<float>(static_cast<int>(v[j])) * __ldg(p.sx + m0 + c + j) * swn;
+          store_y<TY>(static_cast<TY*>(p.Y) + static_cast<long long>(m0 + c + j) * p.ldy + n, f);
+        }
+      }
+    }
+  }
+  if constexpr (S > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp >= 2 && n < p.N) {
+      for (int slot = 0; slot * S + rank < cols; ++slot) {
+        int sum = 0;
+#pragma unroll
+        for (int r = 0; r < S; ++r) sum += part[(r * (BM / S) + slot) * kI8BlockN + row];
+        const int m = m0 + slot * S + rank;
+        store_y<TY>(static_cast<TY*>(p.Y) + static_cast<long long>(m) * p.ldy + n, static_cast<float>(sum) * __ldg(p.sx + m) * swn);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) drain_delay();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- launchers
+// Shared-memory limit of a kernel, raised once per device.
+template <typename Kernel>
+static cudaError_t allow_smem(Kernel kernel, int bytes, unsigned long long& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && ((__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev) & 1ull)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
+  return e;
+}
+
+static int maps_wx(CUtensorMap& tw, CUtensorMap& tx, const void* xq, const void* wq, const Int8GemmParams& p,
+                   long long ldx, long long ldw, int bm) {
+  int r = make_tmap_2d(&tw, wq, 1, p.K, p.N, static_cast<uint64_t>(ldw), kI8BlockK, kI8BlockN, 1);
+  if (r) return r;
+  return make_tmap_2d(&tx, xq, 1, p.K, p.M, static_cast<uint64_t>(ldx), kI8BlockK, bm, 1);
+}
+
+template <int BM, typename TY>
+static int launch_int8(const void* xq, const void* wq, Int8GemmParams p, long long ldx, long long ldw, cudaStream_t stream) {
+  CUtensorMap tw, tx, ty;
+  int r = maps_wx(tw, tx, xq, wq, p, ldx, ldw, BM);
+  if (r) return r;
+  p.tma_out = sizeof(TY) == 2 && p.ldy % 8 == 0 && reinterpret_cast<uintptr_t>(p.Y) % 16 == 0;
+  if (p.tma_out) {
+    r = make_tmap_2d(&ty, p.Y, 2, p.N, p.M, static_cast<uint64_t>(p.ldy) * 2, 32, 64, 0);
+    if (r) return r;
+  } else {
+    ty = tw;
+  }
+  static unsigned long long done = 0;
+  cudaError_t e = allow_smem(gemm_int8_kernel<BM, TY>, Int8Smem<BM>::kTotal, done);
+  if (e != cudaSuccess) return -static_cast<int>(e);
+  const long long tiles = static_cast<long long>((p.N + kI8BlockN - 1) / kI8BlockN) * ((p.M + BM - 1) / BM);
+  if (tiles > 0x7FFFFFFFll) return -kErrBadArgument;
+  const int grid = tiles < sm_count() ? static_cast<int>(tiles) : sm_count();
+  gemm_int8_kernel<BM, TY><<<grid, kI8Threads, Int8Smem<BM>::kTotal, stream>>>(tw, tx, ty, p);
+  return -static_cast<int>(cudaGetLastError());
+}
+
+template <int BM, int S, typename TY>
+static int launch_split(const void* xq, const void* wq, const Int8GemmParams& p, long long ldx, long long ldw,
+                        long long tiles, cudaStream_t stream) {
+  CUtensorMap tw, tx;
+  int r = maps_wx(tw, tx, xq, wq, p, ldx, ldw, BM);
+  if (r) return r;
+  static unsigned long long done = 0;
+  cudaError_t e = allow_smem(gemm_int8_split_kernel<BM, S, TY>, Int8SplitSmem<BM>::kTotal, done);
+  if (e != cudaSuccess) return -static_cast<int>(e);
+  if (tiles * S > 0x7FFFFFFFll) return -kErrBadArgument;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * S));
+  cfg.blockDim = dim3(kI8Threads);
+  cfg.dynamicSmemBytes = Int8SplitSmem<BM>::kTotal;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  return -static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_split_kernel<BM, S, TY>, tw, tx, p));
+}
+
+template <int BM, typename TY>
+static int run_split(const void* xq, const void* wq, const Int8GemmParams& p, long long ldx, long long ldw, cudaStream_t stream) {
+  const long long tiles = static_cast<long long>((p.N + kI8BlockN - 1) / kI8BlockN) * ((p.M + BM - 1) / BM);
+  const int blocks = (p.K + kI8BlockK - 1) / kI8BlockK;
+  int s = 1;   // enough CTAs for every SM, each with two k blocks at least
+  while (s < 8 && tiles * s < sm_count() && blocks >= 4 * s) s *= 2;
+  switch (s) {
+    case 1: return launch_split<BM, 1, TY>(xq, wq, p, ldx, ldw, tiles, stream);
+    case 2: return launch_split<BM, 2, TY>(xq, wq, p, ldx, ldw, tiles, stream);
+    case 4: return launch_split<BM, 4, TY>(xq, wq, p, ldx, ldw, tiles, stream);
+    default: return launch_split<BM, 8, TY>(xq, wq, p, ldx, ldw, tiles, stream);
+  }
+}
+
+template <typename TY>
+static int run_int8(const void* xq, const void* wq, const Int8GemmParams& p, long long ldx, long long ldw, cudaStream_t stream) {
+  if (p.M <= 16) return run_split<16, TY>(xq, wq, p, ldx, ldw, stream);
+  if (p.M <= 32) return run_split<32, TY>(xq, wq, p, ldx, ldw, stream);
+  if (p.M <= 64) return run_split<64, TY>(xq, wq, p, ldx, ldw, stream);
+  const long long n_tiles = (p.N + kI8BlockN - 1) / kI8BlockN;
+  if (n_tiles * ((p.M + 127) / 128) < sm_count()) return run_split<128, TY>(xq, wq, p, ldx, ldw, stream);
+  if (n_tiles * ((p.M + 255) / 256) < 2 * sm_count()) return launch_int8<128, TY>(xq, wq, p, ldx, ldw, stream);
+  return launch_int8<256, TY>(xq, wq, p, ldx, ldw, stream);
+}
+
+}  // namespace stb
+
+using namespace stb;
+
+// xq [M][K], wq [N][K] int8 (row strides ldx, ldw bytes, multiples of 16; bases 16-byte aligned), sx [M], sw [N] fp32,
+// Y [M][N] bf16 or fp32 (row stride ldy elements).
+extern "C" int stb_gemm_int8(const void* xq, const float* sx, const void* wq, const float* sw, void* Y, int M, int N,
+                             int K, long long ldx, long long ldw, long long ldy, int out_f32, int* status,
+                             cudaStream_t stream) {
+  if (M <= 0 || N <= 0) return 0;
+  if (K <= 0 || K > 131071 || (ldx & 15) || (ldw & 15) || ldx < K || ldw < K || ldy < N ||
+      (reinterpret_cast<uintptr_t>(xq) & 15) || (reinterpret_cast<uintptr_t>(wq) & 15))
+    return -kErrBadArgument;
+  Int8GemmParams p{};
+  p.M = M; p.N = N; p.K = K; p.ldy = ldy; p.sx = sx; p.sw = sw; p.Y = Y; p.status = status;
+  return out_f32 ? run_int8<float>(xq, wq, p, ldx, ldw, stream) : run_int8<__nv_bfloat16>(xq, wq, p, ldx, ldw, stream);
+}

@@ -1,0 +1,287 @@
+// Rows to 8 bits, with the residual add and the RMS norm in front of it, in one pass:
+//
+//     s = bf16(x + delta)            the residual stream, written back        (delta optional)
+//     y = s * rsqrt(mean(s^2) + eps) * (w [+ 1])                              (norm optional: y = s)
+//     int8,  one scale per row        : scale = max|y| / 127,  q = round(y / scale)
+//     e4m3,  one scale per 128 columns: scale = max|y| / 448,  q = e4m3(y / scale)
+//
+// The int8 form feeds stb_gemm_int8, the e4m3 form stb_gemm_fp8_block_scaled.  y stays in fp32 between the norm and
+// its single rounding to 8 bits.  A row (block) without a non-zero value gets scale 1; one that holds an infinity or
+// a NaN gets scale NaN, so that it cannot turn into finite numbers downstream.
+//
+// Memory bound: 2 + 2 bytes read, 2 + 1 written per element.  A row lives in the registers of its threads (16 bytes
+// per vector, packed bf16), so everything is read once; the statistics are one sum and one maximum over the row.
+#include "common.cuh"
+
+#include <cuda_fp8.h>
+
+namespace stb {
+
+constexpr int kNqMaxVec = 4;        // vectors of 8 columns per thread
+constexpr int kNqMaxThreads = 1024; // 1024 * 4 * 8 = 32768 columns
+
+struct NormQuantParams {
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* delta;   // nullptr: no residual add
+  const __nv_bfloat16* w;       // nullptr: no norm
+  __nv_bfloat16* s;             // nullptr: the sum is not kept
+  uint8_t* q;
+  float* scale;
+  long long rows, ldx, ldd, lds, ldq;
+  int H;
+  float eps;
+  int zero_centered;
+};
+
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TPR > 32) {
+    const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+    if (l == 0) red[w] = v;
+    __syncthreads();
+    v = l < TPR / 32 ? red[l] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if constexpr (TPR > 32) {
+    const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+    if (l == 0) red[w] = v;
+    __syncthreads();
+    v = __reduce_max_sync(0xffffffffu, l < TPR / 32 ? red[l] : 0u);
+  }
+  return v;
+}
+
+// Scale and its inverse from the bits of max|y| (compared as integers: NaN is above infinity, which is above every
+// number).  Below 6e-36 max / 448 leaves the range of normal numbers; such values count as zero.
+__device__ __forceinline__ void scale_from_max(uint32_t bits, float steps, float& scale, float& inv) {
+  const float amax = __uint_as_float(bits);
+  if (bits >= 0x7F800000u) { scale = __uint_as_float(0x7FC00000u); inv = 0.f; }
+  else if (amax < 6e-36f) { scale = 1.f; inv = 0.f; }
+  else { scale = __fdiv_rn(amax, steps); inv = __fdiv_rn(steps, amax); }
+}
+
+// 8 columns starting at c of one bf16 row; columns from H on read as zero.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int c, int H) {
+  if constexpr (VEC) {
+    return *reinterpret_cast<const uint4*>(row + c);
+  } else {
+    const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int a = c + 2 * j;
+      u[j] = (a < H ? r[a] : 0u) | (a + 1 < H ? static_cast<uint32_t>(r[a + 1]) << 16 : 0u);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(__nv_bfloat16* row, int c, int H, const uint4& v) {
+  if constexpr (VEC) {
+    *reinterpret_cast<uint4*>(row + c) = v;
+  } else {
+    uint16_t* r = reinterpret_cast<uint16_t*>(row);
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < H) r[c + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8_bytes(uint8_t* row, int c, int H, uint32_t lo, uint32_t hi) {
+  if constexpr (VEC) {
+    *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < H) row[c + j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+  }
+}
+
+__device__ __forceinline__ void widen8(const uint4& u, float (&f)[8]) {
+  f[0] = bf16_lo(u.x); f[1] = bf16_hi(u.x); f[2] = bf16_lo(u.y); f[3] = bf16_hi(u.y);
+  f[4] = bf16_lo(u.z); f[5] = bf16_hi(u.z); f[6] = bf16_lo(u.w); f[7] = bf16_hi(u.w);
+}
+
+// TPR threads share a row (a whole CTA, or one of the CTA's four warps when TPR is 32); NV vectors per thread.
+// VEC: every row starts on a 16-byte boundary and H is a multiple of 8; otherwise element by element.
+template <int TPR, int NV, bool E4M3, bool VEC>
+__global__ void __launch_bounds__(TPR < 128 ? (TPR == 32 ? 128 : TPR) : TPR)
+norm_quant_kernel(const NormQuantParams p) {
+  __shared__ float red_sum[32];
+  __shared__ uint32_t red_max[32];
+  const int tid = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
+  const long long row = TPR == 32 ? static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (TPR == 32 && row >= p.rows) return;     // whole warps leave, and no block barrier follows
+  const __nv_bfloat16* xr = p.x + row * p.ldx;
+  const __nv_bfloat16* dr = p.delta != nullptr ? p.delta + row * p.ldd : nullptr;
+  const int nvec = (p.H + 7) / 8;
+
+  uint4 v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int k = tid + i * TPR;
+    v[i] = k < nvec ? load8<VEC>(xr, k * 8, p.H) : make_uint4(0, 0, 0, 0);
+  }
+  if (dr != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = tid + i * TPR;
+      if (k >= nvec) continue;
+      float a[8], b[8];
+      widen8(v[i], a);
+      widen8(load8<VEC>(dr, k * 8, p.H), b);
+      v[i] = make_uint4(pack_bf16(a[0] + b[0], a[1] + b[1]), pack_bf16(a[2] + b[2], a[3] + b[3]),
+                        pack_bf16(a[4] + b[4], a[5] + b[5]), pack_bf16(a[6] + b[6], a[7] + b[7]));
+    }
+  }
+  if (p.s != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = tid + i * TPR;
+      if (k < nvec) store8<VEC>(p.s + row * p.lds, k * 8, p.H, v[i]);
+    }
+  }
+  float rstd = 1.f;
+  if (p.w != nullptr) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[8];
+      widen8(v[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
+    }
+    rstd = rsqrtf(row_sum<TPR>(ss, red_sum) / p.H + p.eps);
+  }
+  const float woff = p.zero_centered ? 1.f : 0.f;
+
+  // y of one vector, in fp32 (recomputed where it is needed twice: the registers hold the bf16 sum)
+  auto normed = [&](int i, float (&f)[8]) {
+    widen8(v[i], f);
+    if (p.w == nullptr) return;
+    const int k = tid + i * TPR;
+    float g[8];
+    widen8(k < nvec ? load8<VEC>(p.w, k * 8, p.H) : make_uint4(0, 0, 0, 0), g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= rstd * (g[j] + woff);
+  };
+  auto top_of = [](const float (&f)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7FFFFFFFu);
+    return m;
+  };
+  uint8_t* qr = p.q + row * p.ldq;
+  if constexpr (E4M3) {
+    // 128 columns are 16 neighbouring lanes
+    const int kbs = p.H / 128;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = tid + i * TPR;
+      float f[8];
+      normed(i, f);
+      uint32_t m = top_of(f);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float scale, inv;
+      scale_from_max(m, 448.f, scale, inv);
+      if (k >= nvec) continue;
+      uint32_t out[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h] * inv, f[4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h + 2] * inv, f[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+        out[h] = a | (b << 16);
+      }
+      store8_bytes<VEC>(qr, k * 8, p.H, out[0], out[1]);
+      if ((k & 15) == 0) p.scale[row * kbs + (k >> 4)] = scale;
+    }
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[8];
+      normed(i, f);
+      m = max(m, top_of(f));
+    }
+    m = row_max<TPR>(m, red_max);
+    float scale, inv;
+    scale_from_max(m, 127.f, scale, inv);
+    if (tid == 0) p.scale[row] = scale;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = tid + i * TPR;
+      if (k >= nvec) continue;
+      float f[8];
+      normed(i, f);
+      uint32_t out[2] = {0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // |y * inv| <= 127 up to rounding, or y * 0 for the rows without a scale (NaN converts to 0)
+        out[j >> 2] |= (static_cast<uint32_t>(__float2int_rn(f[j] * inv)) & 0xFFu) << (8 * (j & 3));
+      }
+      store8_bytes<VEC>(qr, k * 8, p.H, out[0], out[1]);
+    }
+  }
+}
+
+template <int TPR, bool E4M3, bool VEC>
+static cudaError_t launch_norm_quant(const NormQuantParams& p, int nv, cudaStream_t stream) {
+  const int threads = TPR == 32 ? 128 : TPR;
+  const long long blocks = TPR == 32 ? (p.rows + 3) / 4 : p.rows;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (nv <= 1) norm_quant_kernel<TPR, 1, E4M3, VEC><<<grid, threads, 0, stream>>>(p);
+  else if (nv <= 2) norm_quant_kernel<TPR, 2, E4M3, VEC><<<grid, threads, 0, stream>>>(p);
+  else norm_quant_kernel<TPR, 4, E4M3, VEC><<<grid, threads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <bool E4M3, bool VEC>
+static cudaError_t dispatch_norm_quant(const NormQuantParams& p, cudaStream_t stream) {
+  // Threads per row: two vectors per thread, so that a row's loads are in flight together and an SM holds many rows.
+  const int nvec = (p.H + 7) / 8;
+  if (nvec <= 64) return launch_norm_quant<32, E4M3, VEC>(p, (nvec + 31) / 32, stream);
+  if (nvec <= 128) return launch_norm_quant<64, E4M3, VEC>(p, 2, stream);
+  if (nvec <= 256) return launch_norm_quant<128, E4M3, VEC>(p, 2, stream);
+  if (nvec <= 512) return launch_norm_quant<256, E4M3, VEC>(p, 2, stream);
+  if (nvec <= 1024) return launch_norm_quant<512, E4M3, VEC>(p, 2, stream);
+  return launch_norm_quant<1024, E4M3, VEC>(p, (nvec + 1023) / 1024, stream);
+}
+
+}  // namespace stb
+
+using namespace stb;
+
+// fmt 0: int8 with scale [rows]; fmt 1: e4m3 with scale [rows][H / 128] (H a multiple of 128).  Strides in elements.
+extern "C" int stb_norm_quant(const void* x, const void* delta, const void* w, void* s, void* q, float* scale,
+                              long long rows, int H, long long ldx, long long ldd, long long lds, long long ldq,
+                              float eps, int zero_centered, int fmt, cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  if (H <= 0 || H > kNqMaxThreads * kNqMaxVec * 8 || rows > 0x7FFFFFFFll || (fmt == 1 && H % 128)) return -kErrBadArgument;
+  NormQuantParams p{};
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.delta = static_cast<const __nv_bfloat16*>(delta);
+  p.w = static_cast<const __nv_bfloat16*>(w);
+  p.s = static_cast<__nv_bfloat16*>(s);
+  p.q = static_cast<uint8_t*>(q);
+  p.scale = scale;
+  p.rows = rows; p.ldx = ldx; p.ldd = ldd; p.lds = lds; p.ldq = ldq;
+  p.H = H; p.eps = eps; p.zero_centered = zero_centered;
+  auto on16 = [](const void* t, long long ld) { return t == nullptr || (reinterpret_cast<uintptr_t>(t) % 16 == 0 && ld % 8 == 0); };
+  const bool vec = H % 8 == 0 && on16(x, ldx) && on16(delta, ldd) && on16(s, lds) && on16(w, 0) &&
+                   reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
+  cudaError_t e;
+  if (fmt == 1) e = vec ? dispatch_norm_quant<true, true>(p, stream) : dispatch_norm_quant<true, false>(p, stream);
+  else e = vec ? dispatch_norm_quant<false, true>(p, stream) : dispatch_norm_quant<false, false>(p, stream);
+  return -static_cast<int>(e);
+}

@@ -1,0 +1,382 @@
+"""Distillation from a teacher's top logits, on logits and fused with the LM-head projection.
+
+Per token, with the student's logits ``s [V]`` and ``K`` teacher entries ``(id_j, t_j)`` (logits or log-probabilities:
+a constant per token drops out), at temperature ``tau``::
+
+    q = softmax_j(t / tau)      p = softmax_v(s / tau)      loss = sum_j q_j (log q_j - log p[id_j])
+    d loss / d s_v = (p_v - sum_{j: id_j = v} q_j) / tau
+
+An entry of ``-inf`` is no entry (rows of different length are padded with it, whatever their id), nor is one whose id
+lies outside the vocabulary; ids may repeat.  A token without entries has loss 0 and gradient 0, whatever its logits
+hold, and a token of weight 0 has gradient 0.  The factor ``tau ** 2`` that some recipes put in front is left to the
+caller's weights.
+
+The CUDA path is ``csrc/distill.cu``: a row stays in the registers of a thread-block cluster, so that one read of the
+logits gives the loss and the gradient.  Rows longer than the cluster holds, and vocabularies that are sharded over a
+group, take the same sums in three kernels (statistics, loss, gradient) with the statistics all-reduced in between.
+The reference has no distillation loss; the layout follows its vocab-parallel cross-entropy
+(``steptronoss/core/tensor_parallel/cross_entropy.py:28-166``).
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.distributed as dist
+from torch.autograd.function import once_differentiable
+
+from . import native
+from .cross_entropy import _all_reduce
+from .gemm import count_launch, gemm
+
+MAX_ENTRIES = 1024
+P, I, L, F = native.P, native.I, native.L, native.F
+native.register_signature("stb_distill_row_limit", [I])
+native.register_signature("stb_distill_row", [P, L, P, L, P, I, L, P, L, P, P, P, I, I, I, F, I, I, P])
+native.register_signature("stb_distill_stats", [P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, P])
+native.register_signature("stb_distill_loss", [P, I, L, P, L, P, P, P, I, I, L, F, P])
+native.register_signature("stb_distill_grad", [P, L, P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, I, P])
+
+
+# --------------------------------------------------------------------------------------------------- arguments
+def _group_size(group) -> int:
+    return dist.get_world_size(group) if group is not None else 1
+
+
+def _checked(rows: int, device, teacher_ids, teacher_logits, temperature, what: str):
+    """Teacher entries as ``[rows, K]`` with a contiguous last dimension (ids int32 / int64, logits fp32)."""
+    if teacher_ids.shape != teacher_logits.shape or teacher_ids.dim() < 1:
+        raise ValueError(f"{what}: teacher_ids {tuple(teacher_ids.shape)} and teacher_logits "
+                         f"{tuple(teacher_logits.shape)} differ")
+    K = teacher_ids.shape[-1]
+    if K > MAX_ENTRIES:
+        raise ValueError(f"{what}: {K} teacher entries per token, at most {MAX_ENTRIES} are taken")
+    if math.prod(teacher_ids.shape[:-1]) != rows:
+        raise ValueError(f"{what}: teacher entries for {math.prod(teacher_ids.shape[:-1])} tokens, logits for {rows}")
+    if teacher_ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: teacher_ids are int64 or int32, got {teacher_ids.dtype}")
+    if not teacher_logits.is_floating_point():
+        raise TypeError(f"{what}: teacher_logits are floating point, got {teacher_logits.dtype}")
+    if teacher_logits.requires_grad:
+        raise ValueError(f"{what}: no gradient flows to the teacher, detach teacher_logits")
+    if teacher_ids.device != device or teacher_logits.device != device:
+        raise ValueError(f"{what}: teacher entries on {teacher_ids.device} / {teacher_logits.device}, student on {device}")
+    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
+        raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
+    ids, t = teacher_ids.reshape(rows, K), teacher_logits.reshape(rows, K).float()
+    return (ids if ids.stride(-1) == 1 else ids.contiguous()), (t if t.stride(-1) == 1 else t.contiguous())
+
+
+def _rows_of(logits: torch.Tensor, what: str) -> torch.Tensor:
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits need a vocabulary dimension, got {tuple(logits.shape)}")
+    if logits.is_cuda and logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{what}: logits are bf16 or fp32 on the GPU, got {logits.dtype}")
+    x = logits.reshape(-1, logits.shape[-1])
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def _token_weights(weights, rows: int, device, what: str) -> torch.Tensor:
+    if weights.numel() != rows or weights.device != device:
+        raise ValueError(f"{what}: one weight per token on {device}, got {tuple(weights.shape)} on {weights.device}")
+    return weights.detach().reshape(rows).float().contiguous()
+
+
+# --------------------------------------------------------------------------------------------------- PyTorch statement
+def _teacher_q(ids, t, temperature: float, vocab: int):
+    """``(q, log q, has)``; entries that do not count have q = 0."""
+    t = torch.where((ids >= 0) & (ids < vocab), t, -math.inf) / temperature
+    if t.shape[-1] == 0:
+        return t, t, torch.zeros(t.shape[0], dtype=torch.bool, device=t.device)
+    has = t.amax(-1) != -math.inf
+    logq = torch.log_softmax(torch.where(has.unsqueeze(-1), t, 0.0), dim=-1)
+    return torch.where(has.unsqueeze(-1), logq.exp(), 0.0), logq, has
+
+
+def _statement(logits, ids, t, temperature: float, vocab_start: int, group):
+    """``(loss [T], gradient [T, V] for a unit weight)`` in fp32 (fp64 for fp64 logits) from (a vocab shard of) the logits."""
+    s = (logits if logits.dtype == torch.float64 else logits.float()) / temperature
+    V = s.shape[-1]
+    q, logq, has = _teacher_q(ids, t.to(s.dtype), temperature, V * _group_size(group))
+    top = _all_reduce(s.amax(-1), dist.ReduceOp.MAX, group)
+    e = (s - top.unsqueeze(-1)).exp()
+    total = _all_reduce(e.sum(-1), dist.ReduceOp.SUM, group)
+    local = ids - vocab_start
+    here = (local >= 0) & (local < V) & (q != 0)
+    safe = local.masked_fill(~here, 0).long()
+    picked = _all_reduce(torch.where(here, s.gather(-1, safe), 0.0), dist.ReduceOp.SUM, group)
+    terms = q * (logq - (picked - top.unsqueeze(-1) - total.log().unsqueeze(-1)))
+    loss = torch.where(q != 0, terms, 0.0).sum(-1)
+    grad = (e / total.unsqueeze(-1)).scatter_add(-1, safe, -torch.where(here, q, 0.0)) / temperature
+    return loss, torch.where(has.unsqueeze(-1), grad, 0.0)
+
+
+def _weighted(grad, weights):
+    w = weights.unsqueeze(-1)
+    return torch.where(w == 0, 0.0, grad * w)
+
+
+# --------------------------------------------------------------------------------------------------- kernels
+def _fits_row(V: int, elem: int) -> bool:
+    return V <= native.load().stb_distill_row_limit(elem)
+
+
+def _row_kernel(x, ids, t, temperature, weights=None, grad=None, stats=None):
+    """One pass over whole rows: the loss, and on request the gradient and the statistics."""
+    T, V = x.shape
+    loss = torch.empty(T, dtype=torch.float32, device=x.device)
+    native.check(native.load().stb_distill_row(
+        x.data_ptr(), x.stride(0), native.ptr(grad), grad.stride(0) if grad is not None else 0, ids.data_ptr(),
+        int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0), native.ptr(weights), loss.data_ptr(),
+        native.ptr(stats), T, V, ids.shape[1], 1.0 / temperature, x.element_size(),
+        grad.element_size() if grad is not None else x.element_size(), native.stream_of(x.device)), "distill_row")
+    count_launch()
+    return loss
+
+
+def _stats_kernels(x, ids, t, temperature, vocab_start=0, group=None):
+    """``(loss, statistics)`` of rows of any length, or of the shards of a group."""
+    T, V = x.shape
+    K, vocab = ids.shape[1], V * _group_size(group)
+    lib, st = native.load(), native.stream_of(x.device)
+    stats = torch.empty((T, 4), dtype=torch.float32, device=x.device)
+    picked = torch.empty((T, K), dtype=torch.float32, device=x.device)
+    native.check(lib.stb_distill_stats(
+        x.data_ptr(), x.stride(0), ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(),
+        t.stride(0), stats.data_ptr(), picked.data_ptr(), T, V, K, vocab_start, vocab, 1.0 / temperature,
+        x.element_size(), st), "distill_stats")
+    count_launch()
+    if _group_size(group) > 1:
+        _join_shards(stats, picked, group)
+    loss = torch.empty(T, dtype=torch.float32, device=x.device)
+    native.check(lib.stb_distill_loss(
+        ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0), stats.data_ptr(),
+        picked.data_ptr(), loss.data_ptr(), T, K, vocab, 1.0 / temperature, st), "distill_loss")
+    count_launch()
+    return loss, stats
+
+
+def _join_shards(stats, picked, group) -> None:
+    """Statistics of whole rows from those of the group's vocabulary shards, in place.  The first two columns are
+    ``(top, sum of 2^(c s - top))``; the teacher's columns are equal on all ranks."""
+    top = _all_reduce(stats[:, 0].clone(), dist.ReduceOp.MAX, group)
+    # a shard that holds nothing but -inf has top = -inf and sum 0
+    scaled = torch.where(stats[:, 0] == -math.inf, stats[:, 1], stats[:, 1] * torch.exp2(stats[:, 0] - top))
+    stats[:, 1] = _all_reduce(scaled, dist.ReduceOp.SUM, group)
+    stats[:, 0] = top
+    _all_reduce(picked, dist.ReduceOp.SUM, group)
+
+
+def _grad_kernel(x, ids, t, temperature, weights, stats, grad, vocab_start=0, vocab=None):
+    T, V = x.shape
+    native.check(native.load().stb_distill_grad(
+        x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0), ids.data_ptr(), int(ids.dtype == torch.int64),
+        ids.stride(0), t.data_ptr(), t.stride(0), native.ptr(weights), stats.data_ptr(), T, V, ids.shape[1], vocab_start,
+        V if vocab is None else vocab, 1.0 / temperature, x.element_size(), grad.element_size(),
+        native.stream_of(x.device)), "distill_grad")
+    count_launch()
+
+
+def _loss_and_grad(x, ids, t, temperature, weights, grad, vocab_start=0, group=None):
+    """Loss of the rows of ``x``, their weighted gradient into ``grad`` (which may be ``x``)."""
+    if x.shape[0] == 0:
+        return torch.empty(0, dtype=torch.float32, device=x.device)
+    if _group_size(group) == 1 and vocab_start == 0 and _fits_row(x.shape[1], x.element_size()):
+        return _row_kernel(x, ids, t, temperature, weights, grad)
+    loss, stats = _stats_kernels(x, ids, t, temperature, vocab_start, group)
+    _grad_kernel(x, ids, t, temperature, weights, stats, grad, vocab_start, x.shape[1] * _group_size(group))
+    return loss
+
+
+# --------------------------------------------------------------------------------------------------- logits
+class _TopkDistillationFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, t, temperature, vocab_start, group):
+        x = _rows_of(logits, "topk_distillation")
+        ctx.args = (temperature, vocab_start, group)
+        if not x.is_cuda:
+            loss, grad = _statement(x, ids, t, temperature, vocab_start, group)
+            ctx.save_for_backward(grad)
+        elif x.shape[0] == 0:
+            loss = torch.empty(0, dtype=torch.float32, device=x.device)
+            ctx.save_for_backward(x, ids, t, loss)
+        else:
+            with native.on_device(x.device):
+                if _group_size(group) == 1 and vocab_start == 0 and _fits_row(x.shape[1], x.element_size()):
+                    stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device)
+                    loss = _row_kernel(x, ids, t, temperature, stats=stats)
+                else:
+                    loss, stats = _stats_kernels(x, ids, t, temperature, vocab_start, group)
+            ctx.save_for_backward(x, ids, t, stats)
+        ctx.shape, ctx.dtype = logits.shape, logits.dtype
+        return loss.view(logits.shape[:-1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gloss):
+        temperature, vocab_start, group = ctx.args
+        w = gloss.reshape(-1).float().contiguous()
+        if len(ctx.saved_tensors) == 1:
+            (unit,) = ctx.saved_tensors
+            return _weighted(unit, w).to(ctx.dtype).view(ctx.shape), None, None, None, None, None
+        x, ids, t, stats = ctx.saved_tensors
+        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if x.shape[0]:
+            with native.on_device(x.device):
+                _grad_kernel(x, ids, t, temperature, w, stats, grad, vocab_start, x.shape[1] * _group_size(group))
+        return grad.view(ctx.shape), None, None, None, None, None
+
+
+def topk_distillation(logits, teacher_ids, teacher_logits, temperature: float = 1.0, vocab_start: int = 0, group=None):
+    """Per-token loss ``[...]`` (fp32) of ``logits [..., V]`` against teacher entries ``[..., K]``.
+
+    ``logits`` may be a vocabulary shard of equal size on every rank of ``group``, starting at ``vocab_start``;
+    ``teacher_ids`` are always ids of the whole vocabulary.  Differentiable with respect to ``logits``."""
+    temperature = float(temperature)
+    rows = math.prod(logits.shape[:-1])
+    ids, t = _checked(rows, logits.device, teacher_ids, teacher_logits, temperature, "topk_distillation")
+    return _TopkDistillationFn.apply(logits, ids, t, temperature, int(vocab_start), group)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    def span(x):
+        last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+        return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def topk_distillation_loss_and_grad(logits, teacher_ids, teacher_logits, weights, temperature: float = 1.0, out=None):
+    """``(loss [T] fp32, gradient of sum_t weights[t] * loss[t])`` of ``logits [T, V]`` in one pass over them.
+
+    For loops that feed the gradient straight into the next product instead of going through autograd; no graph is
+    recorded.  ``out`` receives the gradient: ``[T, V]`` of the logits' type, or bf16 for fp32 logits, with any row
+    stride; it may be ``logits`` itself (they are overwritten).  The loss is returned without its weight."""
+    what = "topk_distillation_loss_and_grad"
+    temperature = float(temperature)
+    if logits.dim() != 2:
+        raise ValueError(f"{what}: logits are [T, V], got {tuple(logits.shape)}")
+    x = _rows_of(logits.detach(), what)
+    ids, t = _checked(x.shape[0], x.device, teacher_ids, teacher_logits, temperature, what)
+    w = _token_weights(weights, x.shape[0], x.device, what)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        if out.shape != x.shape or out.device != x.device:
+            raise ValueError(f"{what}: out is {tuple(out.shape)} on {out.device}, logits {tuple(x.shape)} on {x.device}")
+        if out.dtype != x.dtype and not (out.dtype == torch.bfloat16 and x.dtype == torch.float32):
+            raise TypeError(f"{what}: out is {out.dtype} for logits of {x.dtype}")
+        if out.stride(-1) != 1 and out.shape[-1] > 1:
+            raise ValueError(f"{what}: the last dimension of out must be contiguous")
+        if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+            raise ValueError(f"{what}: the rows of out overlap")
+        same = out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype and out.stride() == logits.stride()
+        if x.numel() and not same and _overlap(out, logits):
+            raise ValueError(f"{what}: out overlaps logits without being the same tensor")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: out is part of an autograd graph")
+    if not x.is_cuda:
+        loss, grad = _statement(x, ids, t, temperature, 0, None)
+        with torch.no_grad():
+            out.copy_(_weighted(grad, w).to(out.dtype))
+        return loss, out
+    with native.on_device(x.device):
+        loss = _loss_and_grad(x, ids, t, temperature, w, out)
+    torch.autograd.graph.increment_version(out)
+    return loss, out
+
+
+# --------------------------------------------------------------------------------------------------- LM head
+class _FusedLinearTopkDistillationFn(torch.autograd.Function):
+    """Per block of tokens: fp32 logits from the tcgen05 GEMM, loss and bf16 gradient in one pass over them, dgrad and
+    wgrad GEMMs.  The logits stay fp32 because the loss is a difference of log-probabilities: rounded to bf16, logits
+    of size 20 would carry an error of 0.04 into a divergence that is itself of that size late in training."""
+
+    @staticmethod
+    def forward(ctx, h, w, ids, t, weights, temperature, vocab_start, group, chunk):
+        T, H = h.shape
+        V = w.shape[0]
+        dev = h.device
+        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        main_grad = getattr(w, "main_grad", None) if need_dw else None
+        with native.on_device(dev):
+            loss = torch.empty(T, dtype=torch.float32, device=dev)
+            dh = torch.empty((T, H), dtype=torch.float32, device=dev) if need_dh else None
+            dw = main_grad
+            if need_dw and dw is None:
+                dw = torch.empty((V, H), dtype=torch.float32, device=dev) if T else torch.zeros(
+                    (V, H), dtype=torch.float32, device=dev)
+            rows = min(chunk, T)
+            logits = torch.empty((rows, V), dtype=torch.float32, device=dev)
+            grad = torch.empty((rows, V), dtype=torch.bfloat16, device=dev) if need_dh or need_dw else None
+            for t0 in range(0, T, chunk):
+                n = min(T - t0, chunk)
+                s, hc = logits[:n], h[t0:t0 + n]
+                gemm(hc, w, out=s)
+                args = (s, ids[t0:t0 + n], t[t0:t0 + n], temperature)
+                if grad is None:
+                    if _group_size(group) == 1 and vocab_start == 0 and _fits_row(V, 4):
+                        loss[t0:t0 + n] = _row_kernel(*args)
+                    else:
+                        loss[t0:t0 + n] = _stats_kernels(*args, vocab_start, group)[0]
+                    continue
+                g = grad[:n]
+                loss[t0:t0 + n] = _loss_and_grad(*args, weights[t0:t0 + n], g, vocab_start, group)
+                if need_dh:
+                    gemm(g, w, b_mn_major=True, out=dh[t0:t0 + n])
+                if need_dw:
+                    gemm(g, hc, a_mn_major=True, b_mn_major=True, out=dw, accumulate=main_grad is not None or t0 > 0)
+        ctx.save_for_backward(dh)
+        ctx.dw = None if main_grad is not None else dw
+        ctx.w_ref = w
+        ctx.used_main_grad = main_grad is not None
+        ctx.mark_non_differentiable(loss)
+        return torch.where(weights == 0, 0.0, loss * weights).sum(), loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gloss, _):
+        (dh,) = ctx.saved_tensors
+        gh = gw = None
+        if ctx.needs_input_grad[0]:
+            gh = torch.mul(dh, gloss, out=torch.empty(dh.shape, dtype=torch.bfloat16, device=dh.device))
+        if ctx.needs_input_grad[1]:
+            if ctx.used_main_grad:
+                # dW already sits in main_grad with unit upstream gradient: the loss returned by this function has to
+                # be the quantity that backward() is called on.
+                ctx.w_ref.grad_added_to_main_grad = True
+            else:
+                gw = torch.mul(ctx.dw, gloss, out=torch.empty(ctx.dw.shape, dtype=torch.bfloat16, device=ctx.dw.device))
+        return gh, gw, None, None, None, None, None, None, None
+
+
+def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, temperature: float = 1.0,
+                                   vocab_start: int = 0, group=None, chunk_tokens: int = 2048):
+    """``sum_t weights[t] * loss[t]`` of the logits ``h @ w.T`` with vocab-parallel ``w``, and the per-token loss.
+
+    The counterpart of ``fused_linear_cross_entropy`` for a teacher: ``weights`` holds the loss mask already divided by
+    its normaliser (and times ``temperature ** 2`` where the recipe wants that), so the returned scalar is what
+    ``backward()`` is called on; with ``w.main_grad`` the weight gradient is added there during the forward pass.
+    The per-token loss carries no gradient."""
+    what = "fused_linear_topk_distillation"
+    temperature = float(temperature)
+    if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1]:
+        raise ValueError(f"{what}: h is [T, H] and w [V, H], got {tuple(h.shape)} and {tuple(w.shape)}")
+    if chunk_tokens < 1:
+        raise ValueError(f"{what}: chunk_tokens must be positive, got {chunk_tokens}")
+    if w.device != h.device:
+        raise ValueError(f"{what}: h on {h.device}, w on {w.device}")
+    ids, t = _checked(h.shape[0], h.device, teacher_ids, teacher_logits, temperature, what)
+    wt = _token_weights(weights, h.shape[0], h.device, what)
+    if not h.is_cuda:
+        loss = topk_distillation(torch.nn.functional.linear(h, w), ids, t, temperature, vocab_start, group)
+        return torch.where(wt == 0, 0.0, loss * wt).sum(), loss.detach()
+    if h.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+        raise TypeError(f"{what}: h and w are bf16, got {h.dtype} and {w.dtype}")
+    if w.shape[0] % 8 or w.shape[1] % 8 or w.data_ptr() % 16 or w.stride(1) != 1 or w.stride(0) % 8:
+        raise ValueError(f"{what}: w needs a vocabulary and a hidden size that are multiples of 8 and 16-byte aligned "
+                         f"rows, got {tuple(w.shape)} with strides {w.stride()}")
+    if h.stride(1) != 1 or h.data_ptr() % 16 or h.stride(0) % 8:
+        h = h.contiguous()
+    return _FusedLinearTopkDistillationFn.apply(h, w, ids, t, wt, temperature, int(vocab_start), group, int(chunk_tokens))

@@ -1,0 +1,154 @@
+"""Products of frozen weights in 8-bit integers: one scale per token, one per output channel.
+
+``Y[m, n] = sx[m] * sw[n] * sum_k xq[m, k] * wq[n, k]`` with exact int32 sums (``csrc/gemm_int8_sm100.cu``), rounded
+once to bf16 (or fp32).  A frozen model (a distillation teacher, the reference policy of a PPO run) lays its weights
+out once with ``quantize_rows_int8`` and runs its projections with ``linear_int8``, or with ``gemm_int8`` behind
+``add_rmsnorm_quant``, which already leaves int8 rows.  These operators carry no gradient and say so when one is asked
+for.  The reference runs such models in bf16.
+
+Rows of an 8-bit operand start on 16-byte boundaries (the tensor-map copies of the kernel need that):
+``quantize_rows_int8`` returns a view with such a pitch whatever the width.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import native
+from .gemm import count_launch
+
+INT8_MAX = 127.0
+MAX_K = 131071            # int32 sums of 128 * 128 stay below 2^31
+MAX_ROW = 32768           # widest row of the quantisation kernels
+P, I, L, F = native.P, native.I, native.L, native.F
+native.register_signature("stb_gemm_int8", [P, P, P, P, P, I, I, I, L, L, L, I, P, P])
+native.register_signature("stb_norm_quant", [P, P, P, P, P, P, L, I, L, L, L, L, F, I, I, P])
+
+
+def _no_gradient(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: run frozen models under torch.no_grad() or detach the operands")
+
+
+def pitched_int8(rows: int, width: int, device) -> torch.Tensor:
+    """An uninitialised int8 ``[rows, width]`` whose rows start on 16-byte boundaries."""
+    return torch.empty((rows, (width + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :width]
+
+
+def pitched_like(q: torch.Tensor) -> torch.Tensor:
+    """A copy of int8 rows with a pitch that the product takes."""
+    out = pitched_int8(q.shape[0], q.shape[1], q.device)
+    out.copy_(q)
+    return out
+
+
+# ----------------------------------------------------------------------------------------------- quantisation
+def quantize_rows_int8_reference(x: torch.Tensor):
+    """``x [M, K]`` -> ``(q [M, K] int8, scales [M] fp32)``, ``scale = max|x| / 127`` per row, rounded to nearest even.
+
+    A row of zeros has scale 1; a row with a NaN or an infinity has scale NaN and values 0."""
+    xf = x.float()
+    top = xf.abs().amax(dim=-1) if x.shape[-1] else xf.new_zeros(x.shape[:-1])
+    some, finite = top >= 6e-36, torch.isfinite(top)
+    scale = torch.where(some, top / INT8_MAX, 1.0)
+    q = torch.where((some & finite).unsqueeze(-1), torch.round(xf / scale.unsqueeze(-1)), 0.0).to(torch.int8)
+    return q, torch.where(finite, scale, float("nan"))
+
+
+def quantize_rows_int8(x: torch.Tensor):
+    """bf16 rows ``[M, K]`` to int8 with one scale each: tokens of an activation, or output channels of a weight."""
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"quantize_rows_int8 takes [M, K], got {tuple(x.shape)}")
+    _no_gradient("quantize_rows_int8", x)
+    M, K = x.shape
+    if not x.is_cuda:
+        q, s = quantize_rows_int8_reference(x)
+        return pitched_like(q), s
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"quantize_rows_int8 takes bf16 on the GPU, got {x.dtype}")
+    if K > MAX_ROW:
+        raise ValueError(f"quantize_rows_int8 takes rows of at most {MAX_ROW} columns, got {K}")
+    if x.stride(1) != 1 and K > 1:
+        x = x.contiguous()
+    q = pitched_int8(M, K, x.device)
+    s = torch.empty(M, dtype=torch.float32, device=x.device)
+    if M:
+        with native.on_device(x.device):
+            rc = native.load().stb_norm_quant(x.data_ptr(), None, None, None, q.data_ptr(), s.data_ptr(), M, K, x.stride(0),
+                                              0, 0, q.stride(0), 0.0, 0, 0, native.stream_of(x.device))
+        native.check(rc, f"quantize_rows_int8 M={M} K={K}")
+        count_launch()
+    return q, s
+
+
+def dequantize_rows_int8(q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    return q.float() * s.unsqueeze(-1)
+
+
+# ----------------------------------------------------------------------------------------------- products
+def gemm_int8_reference(xq, sx, wq, sw, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The sums in fp64, where every int8 product sum is exact."""
+    dot = xq.double() @ wq.double().t()
+    return (dot.float() * sx.unsqueeze(-1) * sw.unsqueeze(0)).to(out_dtype)
+
+
+def _rows_aligned(t: torch.Tensor) -> bool:
+    return t.data_ptr() % 16 == 0 and (t.shape[1] == 1 or t.stride(1) == 1) and (
+        t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])
+
+
+def gemm_int8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor,
+              out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``xq [M, K]`` (scales ``sx [M]``) times ``wq [N, K]`` transposed (scales ``sw [N]``) -> ``[M, N]``.
+
+    ``out`` (bf16 or fp32, last dimension contiguous, any row stride) takes the result instead of a new tensor."""
+    if xq.dim() != 2 or wq.dim() != 2 or xq.shape[1] != wq.shape[1]:
+        raise ValueError(f"gemm_int8 takes [M, K] and [N, K], got {tuple(xq.shape)} and {tuple(wq.shape)}")
+    M, K = xq.shape
+    N = wq.shape[0]
+    if xq.dtype != torch.int8 or wq.dtype != torch.int8:
+        raise TypeError(f"gemm_int8 takes int8 operands, got {xq.dtype} and {wq.dtype}")
+    if sx.dtype != torch.float32 or sw.dtype != torch.float32 or sx.shape != (M,) or sw.shape != (N,):
+        raise ValueError(f"gemm_int8 takes fp32 scales [{M}] and [{N}], got {sx.dtype} {tuple(sx.shape)} and "
+                         f"{sw.dtype} {tuple(sw.shape)}")
+    if any(t.device != xq.device for t in (sx, wq, sw)):
+        raise ValueError("gemm_int8: operands on different devices")
+    if not 1 <= K <= MAX_K:
+        raise ValueError(f"gemm_int8 takes 1 <= K <= {MAX_K}, got {K}")
+    if out is not None:
+        out_dtype = out.dtype
+        if out.shape != (M, N) or out.device != xq.device or (N > 1 and out.stride(1) != 1) or (
+                M > 1 and out.stride(0) < N):
+            raise ValueError(f"gemm_int8: out must be [{M}, {N}] on {xq.device} with separate rows and a contiguous last "
+                             f"dimension, got {tuple(out.shape)} with strides {out.stride()} on {out.device}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"gemm_int8 writes bf16 or fp32, not {out_dtype}")
+    _no_gradient("gemm_int8", sx, sw, out)
+    if not xq.is_cuda:
+        res = gemm_int8_reference(xq, sx, wq, sw, out_dtype)
+        return res if out is None else out.copy_(res)
+    for name, t in (("xq", xq), ("wq", wq)):
+        if t.shape[0] and not _rows_aligned(t):
+            raise ValueError(f"gemm_int8: rows of {name} must start on 16-byte boundaries and be contiguous, got strides "
+                             f"{t.stride()} (quantize_rows_int8 returns such rows, pitched_like makes them)")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=xq.device)
+    if M and N:
+        sx, sw = sx.contiguous(), sw.contiguous()
+        with native.on_device(xq.device):
+            rc = native.load().stb_gemm_int8(
+                xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, xq.stride(0),
+                wq.stride(0), out.stride(0) if M > 1 else max(out.stride(0), N), int(out_dtype == torch.float32),
+                native.status_word(xq.device).data_ptr(), native.stream_of(xq.device))
+        native.check(rc, f"gemm_int8 M={M} N={N} K={K}")
+        count_launch()
+    return out
+
+
+def linear_int8(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x @ dequantised(w).T`` for bf16 ``x [..., K]``: its rows are quantised on the fly."""
+    _no_gradient("linear_int8", x, sw)
+    if x.dim() < 1 or wq.dim() != 2 or x.shape[-1] != wq.shape[1]:
+        raise ValueError(f"linear_int8 takes [..., K] and [N, K], got {tuple(x.shape)} and {tuple(wq.shape)}")
+    q, s = quantize_rows_int8(x.reshape(-1, x.shape[-1]))
+    y = gemm_int8(q, s, wq, sw, out_dtype=out_dtype or torch.bfloat16)
+    return y.view(*x.shape[:-1], wq.shape[0])

@@ -7,6 +7,7 @@ implementation.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from pathlib import Path
@@ -142,6 +143,23 @@ def stream() -> int:
     if _DEVICE_INDEX is None:
         _DEVICE_INDEX = torch.cuda.current_device()
     return _RAW_STREAM(_DEVICE_INDEX)
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (a launch goes to the current device); nothing to enter when it
+    already is."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def stream_of(device: torch.device) -> int:
+    """The raw handle of the current stream of ``device``, for operators that go by their operands' device."""
+    index = torch.cuda.current_device() if device.index is None else device.index
+    if _RAW_STREAM is None:
+        return torch.cuda.current_stream(index).cuda_stream
+    return _RAW_STREAM(index)
 
 
 _ERRORS = {

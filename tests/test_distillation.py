@@ -1,0 +1,552 @@
+"""Distillation from a teacher's top logits: the statement on CPU, two vocabulary shards on gloo ranks, and the sm_100a
+kernels against the definition in 64 bits."""
+import math
+import os
+
+import pytest
+import torch
+import torch.multiprocessing as mp
+
+from tests.dist_helpers import free_port
+
+INF = math.inf
+
+
+def oracle(logits, ids, teacher, tau, vocab=None, weights=None):
+    """Loss [T], gradient [T, V] of sum_t w_t loss_t, p and q per token, from the definition, in 64 bits."""
+    s = logits.double().cpu() / tau
+    T, V = s.shape
+    t = teacher.double().cpu() / tau
+    ids = ids.long().cpu()
+    w = torch.ones(T, dtype=torch.float64) if weights is None else weights.double().cpu()
+    inside = (ids >= 0) & (ids < (vocab or V))
+    t = torch.where(inside, t, -INF)
+    loss = torch.zeros(T, dtype=torch.float64)
+    q_all = torch.zeros(T, V, dtype=torch.float64)
+    logp = torch.log_softmax(s, -1)
+    p = logp.exp()
+    has = torch.zeros(T, dtype=torch.bool)
+    for r in range(T):
+        keep = t[r] > -INF
+        if not keep.any():
+            continue
+        has[r] = True
+        logq = torch.log_softmax(t[r][keep], -1)
+        q = logq.exp()
+        i = ids[r][keep]
+        d = logq - logp[r][i]
+        loss[r] = (q * torch.where(q > 0, d, 0.0)).sum()
+        q_all[r].index_add_(0, i, q)
+    live = (has & (w != 0)).unsqueeze(1)
+    grad = torch.where(live, (p - q_all) / tau * w.unsqueeze(1), 0.0)
+    return loss, grad, p, q_all
+
+
+def bounds(logits, teacher, tau, p, q, grad, w, out_dtype):
+    """Largest error of loss and gradient by arithmetic, u = 2^-24 per fp32 rounding.  Exponents in units of log2 reach
+    A; an exponent of size A is off by 2 A u after its products, ex2 and lg2 by 4 u; a row's sum is a chain of at most
+    200 additions.  So p is off by (2A + 212) u of itself, q by (2A + 48) u, the logarithms by (4A + 212) u, and q
+    enters the loss times a difference of logarithms of at most 2A."""
+    u = 2.0 ** -24
+    fin = lambda x: x.double()[torch.isfinite(x.double())]
+    span = lambda x: float((x.max() - x.min())) if x.numel() else 0.0
+    A = 1.4427 * max(span(fin(logits)), span(fin(teacher)), float(fin(logits).abs().max()), 1.0) / tau + 20
+    ep, eq = (2 * A + 212) * u, (2 * A + 48) * u
+    loss_tol = (4 * A + 212) * u + 2 * A * eq
+    half_step = torch.finfo(out_dtype).eps / 2
+    grad_tol = w.abs().unsqueeze(1) / tau * (p * ep + q * eq) * 1.01 + grad.abs() * half_step + 1e-37
+    return loss_tol, grad_tol
+
+
+def make(T, V, K, seed=0, dtype=torch.float32, device="cpu", spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn(T, V, generator=g) * spread).to(dtype)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(T)]) if K <= V else torch.randint(
+        0, V, (T, K), generator=g)
+    teacher = torch.randn(T, K, generator=g) * spread
+    weights = torch.rand(T, generator=g) + 0.5
+    return [x.to(device) for x in (logits, ids, teacher, weights)]
+
+
+def check(loss, grad, logits, ids, teacher, weights, tau):
+    want, wgrad, p, q = oracle(logits, ids, teacher, tau, weights=weights)
+    loss_tol, grad_tol = bounds(logits.cpu(), teacher.cpu(), tau, p, q, wgrad, weights.double().cpu(), grad.dtype)
+    assert loss.dtype == torch.float32
+    assert (loss.double().cpu() - want).abs().max() <= loss_tol
+    assert ((grad.double().cpu() - wgrad).abs() <= grad_tol).all()
+
+
+# --------------------------------------------------------------------------------------------------------- CPU
+@pytest.mark.parametrize("tau", [1.0, 0.5, 4.0])
+def test_statement_follows_the_definition(tau):
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(7, 53, 6)
+    teacher[1, 3:] = -INF                 # a shorter row
+    teacher[2] = -INF                     # a row without entries
+    ids[3, 1] = ids[3, 0]                 # the same id twice
+    ids[4, 2], ids[4, 3] = -1, 53         # ids outside the vocabulary
+    w[5] = 0.0
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w, tau)
+    check(loss, grad, logits, ids, teacher, w, tau)
+    assert loss[2] == 0 and grad[2].eq(0).all() and grad[5].eq(0).all()
+    x = logits.clone().requires_grad_()
+    per_token = topk_distillation(x, ids, teacher, tau)
+    (per_token * w).sum().backward()
+    assert torch.equal(per_token.detach(), loss) and torch.allclose(x.grad, grad, atol=1e-7)
+    lead = topk_distillation(logits.view(1, 7, 53), ids.view(1, 7, 6), teacher.view(1, 7, 6), tau)
+    assert lead.shape == (1, 7) and torch.equal(lead[0], loss)
+
+
+def test_gradient_agrees_with_differences():
+    from steptronoss_b200.ops import topk_distillation
+
+    logits, ids, teacher, _ = make(4, 11, 5, dtype=torch.float64)
+    ids[0, 1] = ids[0, 0]
+    teacher[1, 2:] = -INF
+    torch.autograd.gradcheck(lambda x: topk_distillation(x, ids, teacher, 1.5), logits.requires_grad_(), atol=1e-6)
+
+
+def test_rows_that_do_not_count_may_hold_anything():
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(4, 9, 3)
+    logits[0], logits[1, 2] = math.nan, -INF
+    teacher[0] = -INF
+    logits[2] = math.nan
+    w[2] = 0.0
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    assert loss[0] == 0 and grad[0].eq(0).all() and grad[2].eq(0).all() and grad[1].isfinite().all()
+    x = logits.clone().requires_grad_()
+    loss = topk_distillation(x, ids, teacher)
+    loss[torch.tensor([0, 1, 3])].sum().backward()
+    assert x.grad[0].eq(0).all() and x.grad[2].eq(0).all() and x.grad.isfinite().all()
+
+
+def test_zero_entries_and_zero_tokens():
+    from steptronoss_b200.ops import fused_linear_topk_distillation, topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(3, 9, 2)
+    loss, grad = topk_distillation_loss_and_grad(logits, ids[:, :0], teacher[:, :0], w)
+    assert loss.eq(0).all() and grad.eq(0).all()
+    loss, grad = topk_distillation_loss_and_grad(logits[:0], ids[:0], teacher[:0], w[:0])
+    assert loss.shape == (0,) and grad.shape == (0, 9)
+    total, tok = fused_linear_topk_distillation(torch.zeros(0, 8), torch.zeros(16, 8), ids[:0], teacher[:0], w[:0])
+    assert total == 0 and tok.shape == (0,)
+
+
+def test_in_place_and_given_output():
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(5, 33, 4)
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    wide = torch.full((5, 40), 7.0, dtype=torch.bfloat16)
+    loss2, out = topk_distillation_loss_and_grad(logits, ids, teacher, w, out=wide[:, :33])
+    assert torch.equal(loss, loss2) and torch.equal(out, grad.to(torch.bfloat16)) and wide[:, 33:].eq(7).all()
+    buf = logits.clone()
+    loss3, out = topk_distillation_loss_and_grad(buf, ids, teacher, w, out=buf)
+    assert out.data_ptr() == buf.data_ptr() and torch.equal(loss, loss3) and torch.equal(buf, grad)
+
+
+def test_fused_head_on_cpu_is_the_head_and_the_loss():
+    from steptronoss_b200.ops import fused_linear_topk_distillation, topk_distillation
+
+    torch.manual_seed(0)
+    _, ids, teacher, w = make(6, 24, 4)
+    h, head = torch.randn(6, 8, requires_grad=True), torch.randn(24, 8, requires_grad=True)
+    total, tok = fused_linear_topk_distillation(h, head, ids, teacher, w, 2.0)
+    got = torch.autograd.grad(total, [h, head])
+    loss = topk_distillation(h @ head.t(), ids, teacher, 2.0)
+    want = torch.autograd.grad((loss * w).sum(), [h, head])
+    assert torch.allclose(tok, loss) and not tok.requires_grad
+    assert all(torch.allclose(a, b, atol=1e-6) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(teacher_ids=torch.zeros(4, 3, dtype=torch.long)), ValueError),
+    (dict(teacher_logits=torch.zeros(3, 2)), ValueError),
+    (dict(teacher_ids=torch.zeros(4, 2)), TypeError),
+    (dict(teacher_logits=torch.zeros(4, 2, dtype=torch.long)), TypeError),
+    (dict(teacher_logits=torch.zeros(4, 2, requires_grad=True)), ValueError),
+    (dict(teacher_ids=torch.zeros(4, 1025, dtype=torch.long), teacher_logits=torch.zeros(4, 1025)), ValueError),
+    (dict(temperature=0.0), ValueError),
+    (dict(temperature=-1.0), ValueError),
+    (dict(temperature=math.nan), ValueError),
+    (dict(temperature=math.inf), ValueError),
+    (dict(weights=torch.ones(3)), ValueError),
+    (dict(logits=torch.zeros(2, 2, 9)), ValueError),
+    (dict(logits=torch.zeros(4, 0)), ValueError),
+    (dict(out=torch.zeros(4, 8)), ValueError),
+    (dict(out=torch.zeros(4, 9, dtype=torch.float16)), TypeError),
+    (dict(out=torch.zeros(9, 4).t()), ValueError),
+    (dict(out=torch.zeros(1, 9).expand(4, 9)), ValueError),
+    (dict(out=torch.zeros(4, 9, requires_grad=True)), ValueError),
+])
+def test_refusals(change, error):
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    args = dict(logits=torch.zeros(4, 9), teacher_ids=torch.zeros(4, 2, dtype=torch.long),
+                teacher_logits=torch.zeros(4, 2), weights=torch.ones(4))
+    topk_distillation_loss_and_grad(**args)
+    with pytest.raises(error):
+        topk_distillation_loss_and_grad(**{**args, **change})
+
+
+def test_refuses_an_output_that_overlaps_the_logits():
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    buf = torch.zeros(100)
+    logits, out = buf[:36].view(4, 9), buf[4:40].view(4, 9)
+    with pytest.raises(ValueError):
+        topk_distillation_loss_and_grad(logits, torch.zeros(4, 2, dtype=torch.long), torch.zeros(4, 2), torch.ones(4), out=out)
+
+
+def test_fused_head_refusals():
+    from steptronoss_b200.ops import fused_linear_topk_distillation as f
+
+    ids, t, w = torch.zeros(4, 2, dtype=torch.long), torch.zeros(4, 2), torch.ones(4)
+    for h, head, more in ((torch.zeros(4, 8), torch.zeros(16, 7), {}), (torch.zeros(1, 4, 8), torch.zeros(16, 8), {}),
+                          (torch.zeros(4, 8), torch.zeros(16, 8), dict(chunk_tokens=0)),
+                          (torch.zeros(5, 8), torch.zeros(16, 8), {})):
+        with pytest.raises(ValueError):
+            f(h, head, ids, t, w, **more)
+
+
+def _shard_worker(rank, world, port, q):
+    os.environ.update(RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank), MASTER_ADDR="127.0.0.1",
+                      MASTER_PORT=str(port))
+    torch.set_num_threads(1)
+    try:
+        import torch.distributed as dist
+
+        from steptronoss_b200.ops import topk_distillation
+
+        dist.init_process_group("gloo", rank=rank, world_size=world)
+        logits, ids, teacher, w = make(6, 16, 5, seed=3)
+        teacher[1, 2:] = -INF
+        teacher[2] = -INF
+        ids[3, 0], ids[4, 1] = 99, ids[4, 0]
+        shard = logits[:, rank * 8:(rank + 1) * 8].clone().requires_grad_()
+        loss = topk_distillation(shard, ids, teacher, 2.0, rank * 8, dist.group.WORLD)
+        (loss * w).sum().backward()
+        q.put((rank, loss.tolist(), shard.grad.tolist(), None))
+        dist.barrier()
+        dist.destroy_process_group()
+    except BaseException:
+        import traceback
+
+        q.put((rank, None, None, traceback.format_exc()))
+        raise
+
+
+def test_two_vocabulary_shards_equal_the_whole():
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = free_port()
+    procs = [ctx.Process(target=_shard_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = {}
+    try:
+        for _ in range(2):
+            rank, loss, grad, err = q.get(timeout=120)
+            assert err is None, err
+            res[rank] = (torch.tensor(loss), torch.tensor(grad))
+    finally:
+        for p in procs:
+            p.join(timeout=30)
+            if p.is_alive():
+                p.kill()
+    logits, ids, teacher, w = make(6, 16, 5, seed=3)
+    teacher[1, 2:] = -INF
+    teacher[2] = -INF
+    ids[3, 0], ids[4, 1] = 99, ids[4, 0]
+    check(res[0][0], torch.cat([res[0][1], res[1][1]], dim=1), logits, ids, teacher, w, 2.0)
+    assert torch.equal(res[0][0], res[1][0])
+
+
+# --------------------------------------------------------------------------------------------------------- GPU
+SHAPES = [(1, 1, 1), (3, 7, 3), (5, 1000, 17), (70, 4099, 33), (2, 50257, 20), (149, 2048, 64), (3, 151936, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,K", SHAPES)
+def test_one_pass_kernel_follows_the_definition(T, V, K, dtype):
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    for tau, id_type in ((1.0, torch.int64), (0.5, torch.int32)):
+        logits, ids, teacher, w = make(T, V, K, dtype=dtype, device="cuda")
+        loss, grad = topk_distillation_loss_and_grad(logits, ids.to(id_type), teacher, w, tau)
+        assert grad.dtype == dtype
+        check(loss, grad, logits, ids, teacher, w, tau)
+        again, grad2 = topk_distillation_loss_and_grad(logits, ids.to(id_type), teacher, w, tau)
+        assert torch.equal(loss, again) and torch.equal(grad, grad2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,K", SHAPES)
+def test_autograd_kernels_follow_the_definition(T, V, K, dtype):
+    from steptronoss_b200.ops import topk_distillation
+
+    logits, ids, teacher, w = make(T, V, K, seed=1, dtype=dtype, device="cuda")
+    x = logits.clone().requires_grad_()
+    loss = topk_distillation(x.view(1, T, V), ids.view(1, T, K), teacher.view(1, T, K), 2.0)
+    (grad,) = torch.autograd.grad(loss, x, w.view(1, T))
+    check(loss.detach().view(T), grad, logits, ids, teacher, w, 2.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masks_repeated_and_foreign_ids_on_the_gpu(dtype):
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    T, V, K = 9, 20000, 40
+    logits, ids, teacher, w = make(T, V, K, seed=2, dtype=dtype, device="cuda")
+    teacher[1, 5:] = -INF
+    teacher[2] = -INF
+    ids[3, 7:20] = ids[3, 6]                       # thirteen entries of one id
+    ids[4, 0], ids[4, 1], ids[4, 2] = -1, V, 2 ** 40
+    w[5] = 0.0
+    logits[6, 100:300] = -INF                      # a masked part of the vocabulary, no entry there
+    ids[6] = torch.arange(1000, 1000 + K, device="cuda")
+    ids[7, 0], ids[7, 1] = 0, V - 1                # the ends of a row
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    check(loss, grad, logits, ids, teacher, w, 1.0)
+    assert loss[2] == 0 and grad[2].eq(0).all() and grad[5].eq(0).all() and grad[6, 100:300].eq(0).all()
+    x = logits.clone().requires_grad_()
+    tok = topk_distillation(x, ids, teacher)
+    (grad2,) = torch.autograd.grad(tok, x, w)
+    check(tok.detach(), grad2, logits, ids, teacher, w, 1.0)
+    # rows that do not count may hold anything; a NaN elsewhere stays in its row and shows
+    logits[2] = math.nan
+    logits[5, 3] = math.nan
+    logits[8, 4] = math.nan
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    assert loss[2] == 0 and grad[2].eq(0).all() and grad[5].eq(0).all()
+    assert loss[8].isnan() and grad[8].isnan().all()
+    rest = [0, 1, 3, 4, 6, 7]
+    assert loss[rest].isfinite().all() and grad[rest].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_infinite_loss_where_the_student_excludes_an_entry():
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(2, 600, 4, device="cuda")
+    logits[0, ids[0, 1]] = -INF
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    assert loss[0] == INF and loss[1].isfinite() and grad.isfinite().all()
+    q = torch.softmax(teacher[0].double(), 0)[1]
+    assert abs(float(grad[0, ids[0, 1]]) + float(q * w[0])) < 1e-6       # p = 0 there
+    logits[1] = -INF
+    assert topk_distillation_loss_and_grad(logits, ids, teacher, w)[0][1].isnan()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strides_alignment_and_in_place(dtype):
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    T, V, K = 6, 5003, 12
+    logits, ids, teacher, w = make(T, V, K, seed=4, dtype=dtype, device="cuda")
+    want_loss, want = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    for pitch, first in ((5008, 0), (5011, 3), (5024, 1)):
+        store = torch.full((T * pitch + 8,), 5.0, dtype=dtype, device="cuda")
+        view = store[first:first + T * pitch].view(T, pitch)[:, :V]
+        view.copy_(logits)
+        out_store = torch.full((T, V + 9), 3.0, dtype=dtype, device="cuda")
+        loss, grad = topk_distillation_loss_and_grad(view, ids, teacher, w, out=out_store[:, 2:2 + V])
+        check(loss, grad, logits, ids, teacher, w, 1.0)
+        assert out_store[:, :2].eq(3).all() and out_store[:, 2 + V:].eq(3).all()
+        if dtype == torch.float32:
+            half = torch.full((T, V + 5), 3.0, dtype=torch.bfloat16, device="cuda")
+            loss, grad = topk_distillation_loss_and_grad(view, ids, teacher, w, out=half[:, 1:1 + V])
+            check(loss, grad, logits, ids, teacher, w, 1.0)
+            assert half[:, 0].eq(3).all() and half[:, 1 + V:].eq(3).all()
+        x = view.detach().requires_grad_()
+        (grad,) = torch.autograd.grad(topk_distillation(x, ids, teacher), x, w)
+        check(want_loss, grad, logits, ids, teacher, w, 1.0)
+        loss, grad = topk_distillation_loss_and_grad(view, ids, teacher, w, out=view)   # last: overwrites the logits
+        check(loss, grad, logits, ids, teacher, w, 1.0)
+        rest = store.clone()
+        rest[first:first + T * pitch].view(T, pitch)[:, :V] = 5.0
+        assert rest.eq(5).all()                                                            # nothing between the rows
+    t_wide = torch.full((T, K + 3), 9.0, device="cuda")
+    t_wide[:, 2:2 + K] = teacher
+    i_wide = torch.zeros(T, K + 1, dtype=torch.int32, device="cuda")
+    i_wide[:, 1:] = ids
+    loss, grad = topk_distillation_loss_and_grad(logits, i_wide[:, 1:], t_wide[:, 2:2 + K], w)
+    assert torch.equal(loss, want_loss) and torch.equal(grad, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 330001), (torch.float32, 163900)])
+def test_rows_longer_than_a_cluster_holds(dtype, V):
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+    from steptronoss_b200.ops.distillation import _fits_row
+
+    assert not _fits_row(V, dtype.itemsize) and _fits_row(V // 2, dtype.itemsize)
+    logits, ids, teacher, w = make(2, V, 30, seed=5, dtype=dtype, device="cuda")
+    ids[0, 3] = ids[0, 2]
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w, 0.7)
+    # this kernel adds V / 512 exponentials per thread: a longer chain than the bound's 200, of V / 512 + 16
+    assert V / 512 + 16 < 700
+    want, wgrad, p, q = oracle(logits, ids, teacher, 0.7, weights=w)
+    loss_tol, grad_tol = bounds(logits.cpu(), teacher.cpu(), 0.7, p, q, wgrad, w.double().cpu(), dtype)
+    more = 500 * 2.0 ** -24
+    assert (loss.double().cpu() - want).abs().max() <= loss_tol + more
+    assert ((grad.double().cpu() - wgrad).abs() <= grad_tol + w.double().cpu()[:, None] / 0.7 * p * more).all()
+    buf = logits.clone()
+    loss2, _ = topk_distillation_loss_and_grad(buf, ids, teacher, w, 0.7, out=buf)
+    assert torch.equal(loss, loss2) and torch.equal(buf, grad)
+    x = logits.clone().requires_grad_()
+    tok = topk_distillation(x, ids, teacher, 0.7)
+    assert torch.equal(tok.detach(), loss)
+
+
+@pytest.mark.gpu
+def test_many_entries():
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(3, 1500, 1024, device="cuda")
+    ids[1] = ids[1] % 40                            # every id about 25 times
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    check(loss, grad, logits, ids, teacher, w, 1.0)
+    loss, grad = topk_distillation_loss_and_grad(logits, ids[:, :0], teacher[:, :0], w)
+    assert loss.eq(0).all() and grad.eq(0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_shards_joined_by_hand_equal_the_whole(dtype):
+    """The kernels of a sharded vocabulary, the all-reduces done on one device."""
+    from steptronoss_b200.ops import distillation as d
+    from steptronoss_b200.ops import native
+
+    T, V, K, tau, parts = 5, 3000, 21, 2.0, 3
+    logits, ids, teacher, w = make(T, V, K, seed=6, dtype=dtype, device="cuda")
+    ids[0, 0] = V + 5
+    teacher[1] = -INF
+    logits[2, :1000] = -INF                        # one shard without any probability
+    ids[2] = torch.arange(1500, 1500 + K, device="cuda")
+    lib, st = native.load(), native.stream_of(logits.device)
+    stats, picked = [], []
+    for r in range(parts):
+        x = logits[:, r * 1000:(r + 1) * 1000]
+        s = torch.empty(T, 4, device="cuda")
+        pk = torch.empty(T, K, device="cuda")
+        assert lib.stb_distill_stats(x.data_ptr(), x.stride(0), ids.data_ptr(), 1, ids.stride(0), teacher.data_ptr(), K,
+                                     s.data_ptr(), pk.data_ptr(), T, 1000, K, r * 1000, V, 1 / tau, x.element_size(), st) == 0
+        stats.append(s)
+        picked.append(pk)
+    top = torch.stack([s[:, 0] for s in stats]).amax(0)
+    whole = stats[0].clone()
+    whole[:, 1] = sum(torch.where(s[:, 0] == -INF, s[:, 1], s[:, 1] * torch.exp2(s[:, 0] - top)) for s in stats)
+    whole[:, 0] = top
+    together = sum(picked)
+    loss = torch.empty(T, device="cuda")
+    assert lib.stb_distill_loss(ids.data_ptr(), 1, ids.stride(0), teacher.data_ptr(), K, whole.data_ptr(),
+                                together.data_ptr(), loss.data_ptr(), T, K, V, 1 / tau, st) == 0
+    grad = torch.empty_like(logits)
+    for r in range(parts):
+        sl = slice(r * 1000, (r + 1) * 1000)
+        d._grad_kernel(logits[:, sl], ids, teacher, tau, w, whole, grad[:, sl], r * 1000, V)
+    check(loss, grad, logits, ids, teacher, w, tau)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V,chunk", [(5, 64, 1000, 2048), (300, 128, 5000, 128), (257, 256, 151936, 100)])
+def test_fused_head_follows_the_definition(T, H, V, chunk):
+    from steptronoss_b200.ops import fused_linear_topk_distillation, native
+
+    torch.manual_seed(0)
+    K, tau = 16, 2.0
+    _, ids, teacher, w = make(T, V, K, seed=7, device="cuda")
+    teacher[1] = -INF
+    w[2] = 0.0
+    h = torch.randn(T, H, device="cuda").to(torch.bfloat16).requires_grad_()
+    head = (torch.randn(V, H, device="cuda") * 3 / H ** 0.5).to(torch.bfloat16).requires_grad_()
+    total, tok = fused_linear_topk_distillation(h, head, ids, teacher, w, tau, chunk_tokens=chunk)
+    dh, dw = torch.autograd.grad(total, [h, head], retain_graph=True)
+    dh2, _ = torch.autograd.grad(total, [h, head], torch.tensor(0.5, device="cuda"))
+    torch.cuda.synchronize()
+    native.raise_if_kernel_error()
+    logits = h.detach().double() @ head.detach().double().t()
+    want, g, p, q = oracle(logits, ids, teacher, tau, weights=w)
+    # the logits are sums of H products of size 3 sqrt(H) / sqrt(H) in fp32: H roundings of 2^-24 of sum |a b| at most
+    mag = float((h.detach().double().abs() @ head.detach().double().abs().t()).max())
+    e = H * 2.0 ** -24 * mag / tau
+    loss_tol, _ = bounds(logits.cpu(), teacher.cpu(), tau, p, q, g, w.double().cpu(), torch.bfloat16)
+    assert (tok.double().cpu() - want).abs().max() <= loss_tol + 2 * e
+    assert abs(float(total) - float((want * w.double().cpu()).sum())) <= (loss_tol + 2 * e) * float(w.sum()) * 1.01
+    # gradient rows are rounded to bf16 (2^-8 of each), the products summed in fp32 and rounded once more
+    for got, a, b in ((dh, g, head.detach().double().cpu()), (dw, g.t(), h.detach().double().cpu())):
+        exact, size = a @ b, a.abs() @ b.abs()
+        tol = size * (2.0 ** -8 + 2 * e + 1e-4) + exact.abs() * 2.0 ** -8 + 1e-30
+        assert ((got.double().cpu() - exact).abs() <= tol).all()
+    assert torch.allclose(dh2.float(), 0.5 * dh.float(), rtol=2.0 ** -8, atol=0)
+    with torch.no_grad():
+        total2, tok2 = fused_linear_topk_distillation(h, head, ids, teacher, w, tau, chunk_tokens=chunk)
+    assert torch.equal(tok, tok2) and total2 == total
+
+
+@pytest.mark.gpu
+def test_fused_head_adds_into_main_grad():
+    from steptronoss_b200.ops import fused_linear_topk_distillation
+
+    torch.manual_seed(0)
+    T, H, V, K = 90, 64, 512, 8
+    _, ids, teacher, w = make(T, V, K, seed=8, device="cuda")
+    h = torch.randn(T, H, device="cuda").to(torch.bfloat16)
+    head = torch.nn.Parameter((torch.randn(V, H, device="cuda") * 0.3).to(torch.bfloat16))
+    total, _ = fused_linear_topk_distillation(h, head, ids, teacher, w, chunk_tokens=32)
+    total.backward()
+    plain = head.grad.float().clone()
+    head.grad, head.main_grad = None, torch.ones(V, H, device="cuda")
+    total, _ = fused_linear_topk_distillation(h, head, ids, teacher, w, chunk_tokens=32)
+    total.backward()
+    assert head.grad is None and head.grad_added_to_main_grad
+    assert torch.allclose(head.main_grad - 1, plain, rtol=2.0 ** -8, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_kernels_on_a_side_stream_and_in_a_graph():
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(17, 30000, 24, dtype=torch.bfloat16, device="cuda")
+    want_loss, want = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(loss, want_loss) and torch.equal(grad, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    logits.mul_(0.5)
+    want_loss, want = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want_loss) and torch.equal(grad, want)
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    from steptronoss_b200.ops import fused_linear_topk_distillation, topk_distillation
+
+    _, ids, teacher, w = make(4, 16, 2, device="cuda")
+    with pytest.raises(TypeError):
+        topk_distillation(torch.zeros(4, 16, dtype=torch.float16, device="cuda"), ids, teacher)
+    with pytest.raises(ValueError):
+        topk_distillation(torch.zeros(4, 16, device="cuda"), ids.cpu(), teacher)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(TypeError):
+        fused_linear_topk_distillation(bf(4, 8).float(), bf(16, 8), ids, teacher, w)
+    with pytest.raises(ValueError):
+        fused_linear_topk_distillation(bf(4, 8), bf(17, 8), ids, teacher, w)
+    with pytest.raises(ValueError):
+        fused_linear_topk_distillation(bf(4, 12), bf(16, 12), ids, teacher, w)
