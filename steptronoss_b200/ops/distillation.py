@@ -11,7 +11,7 @@ lies outside the vocabulary; ids may repeat.  A token without entries has loss 0
 hold, and a token of weight 0 has gradient 0.  The factor ``tau ** 2`` that some recipes put in front is left to the
 caller's weights.
 
-The CUDA path is ``csrc/distill.cu``: a row stays in the registers of a thread-block cluster, so that one read of the
+The CUDA path is ``csrc/distill.cu``: a row stays in the shared memory of a thread-block cluster, so that one read of the
 logits gives the loss and the gradient.  Rows longer than the cluster holds, and vocabularies that are sharded over a
 group, take the same sums in three kernels (statistics, loss, gradient) with the statistics all-reduced in between.
 The reference has no distillation loss; the layout follows its vocab-parallel cross-entropy
@@ -32,7 +32,7 @@ from .gemm import count_launch, gemm
 MAX_ENTRIES = 1024
 P, I, L, F = native.P, native.I, native.L, native.F
 native.register_signature("stb_distill_row_limit", [I])
-native.register_signature("stb_distill_row", [P, L, P, L, P, I, L, P, L, P, P, P, I, I, I, F, I, I, P])
+native.register_signature("stb_distill_row", [P, L, P, L, P, I, L, P, L, P, P, P, I, I, I, F, I, I, P, P])
 native.register_signature("stb_distill_stats", [P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, P])
 native.register_signature("stb_distill_loss", [P, I, L, P, L, P, P, P, I, I, L, F, P])
 native.register_signature("stb_distill_grad", [P, L, P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, I, P])
@@ -43,42 +43,50 @@ def _group_size(group) -> int:
     return dist.get_world_size(group) if group is not None else 1
 
 
-def _checked(rows: int, device, teacher_ids, teacher_logits, temperature, what: str):
-    """Teacher entries as ``[rows, K]`` with a contiguous last dimension (ids int32 / int64, logits fp32)."""
-    if teacher_ids.shape != teacher_logits.shape or teacher_ids.dim() < 1:
-        raise ValueError(f"{what}: teacher_ids {tuple(teacher_ids.shape)} and teacher_logits "
-                         f"{tuple(teacher_logits.shape)} differ")
-    K = teacher_ids.shape[-1]
+def _checked(rows: int, index: int, teacher_ids, teacher_logits, temperature, what: str):
+    """Teacher entries as ``[rows, K]`` with a contiguous last dimension (ids int32 / int64, logits fp32); ``index`` is
+    the student's device."""
+    shape = teacher_ids.shape
+    if shape != teacher_logits.shape or len(shape) < 1:
+        raise ValueError(f"{what}: teacher_ids {tuple(shape)} and teacher_logits {tuple(teacher_logits.shape)} differ")
+    K = shape[-1]
     if K > MAX_ENTRIES:
         raise ValueError(f"{what}: {K} teacher entries per token, at most {MAX_ENTRIES} are taken")
-    if math.prod(teacher_ids.shape[:-1]) != rows:
-        raise ValueError(f"{what}: teacher entries for {math.prod(teacher_ids.shape[:-1])} tokens, logits for {rows}")
-    if teacher_ids.dtype not in (torch.int64, torch.int32):
+    if math.prod(shape[:-1]) != rows:
+        raise ValueError(f"{what}: teacher entries for {math.prod(shape[:-1])} tokens, logits for {rows}")
+    if teacher_ids.dtype != torch.int64 and teacher_ids.dtype != torch.int32:
         raise TypeError(f"{what}: teacher_ids are int64 or int32, got {teacher_ids.dtype}")
     if not teacher_logits.is_floating_point():
         raise TypeError(f"{what}: teacher_logits are floating point, got {teacher_logits.dtype}")
     if teacher_logits.requires_grad:
         raise ValueError(f"{what}: no gradient flows to the teacher, detach teacher_logits")
-    if teacher_ids.device != device or teacher_logits.device != device:
-        raise ValueError(f"{what}: teacher entries on {teacher_ids.device} / {teacher_logits.device}, student on {device}")
+    if teacher_ids.get_device() != index or teacher_logits.get_device() != index:
+        raise ValueError(f"{what}: teacher entries on {teacher_ids.device} / {teacher_logits.device}, not on the student's "
+                         "device")
     if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
         raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
-    ids, t = teacher_ids.reshape(rows, K), teacher_logits.reshape(rows, K).float()
-    return (ids if ids.stride(-1) == 1 else ids.contiguous()), (t if t.stride(-1) == 1 else t.contiguous())
+    if len(shape) != 2:
+        teacher_ids, teacher_logits = teacher_ids.reshape(rows, K), teacher_logits.reshape(rows, K)
+    if teacher_logits.dtype != torch.float32:
+        teacher_logits = teacher_logits.float()
+    return (teacher_ids if teacher_ids.stride(1) == 1 else teacher_ids.contiguous(),
+            teacher_logits if teacher_logits.stride(1) == 1 else teacher_logits.contiguous())
 
 
 def _rows_of(logits: torch.Tensor, what: str) -> torch.Tensor:
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits need a vocabulary dimension, got {tuple(logits.shape)}")
-    if logits.is_cuda and logits.dtype not in (torch.bfloat16, torch.float32):
+    if logits.is_cuda and logits.dtype != torch.bfloat16 and logits.dtype != torch.float32:
         raise TypeError(f"{what}: logits are bf16 or fp32 on the GPU, got {logits.dtype}")
-    x = logits.reshape(-1, logits.shape[-1])
-    return x if x.stride(-1) == 1 else x.contiguous()
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    return x if x.stride(1) == 1 else x.contiguous()
 
 
-def _token_weights(weights, rows: int, device, what: str) -> torch.Tensor:
-    if weights.numel() != rows or weights.device != device:
-        raise ValueError(f"{what}: one weight per token on {device}, got {tuple(weights.shape)} on {weights.device}")
+def _token_weights(weights, rows: int, index: int, what: str) -> torch.Tensor:
+    if weights.numel() != rows or weights.get_device() != index:
+        raise ValueError(f"{what}: one weight per token on the student's device, got {tuple(weights.shape)} on {weights.device}")
+    if weights.dtype == torch.float32 and weights.dim() == 1 and not weights.requires_grad and weights.is_contiguous():
+        return weights
     return weights.detach().reshape(rows).float().contiguous()
 
 
@@ -117,19 +125,29 @@ def _weighted(grad, weights):
 
 
 # --------------------------------------------------------------------------------------------------- kernels
+_ROW_LIMIT: dict[int, int] = {}
+
+
 def _fits_row(V: int, elem: int) -> bool:
-    return V <= native.load().stb_distill_row_limit(elem)
+    limit = _ROW_LIMIT.get(elem)
+    if limit is None:
+        limit = _ROW_LIMIT[elem] = native.load().stb_distill_row_limit(elem)
+    return V <= limit
 
 
 def _row_kernel(x, ids, t, temperature, weights=None, grad=None, stats=None):
     """One pass over whole rows: the loss, and on request the gradient and the statistics."""
     T, V = x.shape
-    loss = torch.empty(T, dtype=torch.float32, device=x.device)
-    native.check(native.load().stb_distill_row(
-        x.data_ptr(), x.stride(0), native.ptr(grad), grad.stride(0) if grad is not None else 0, ids.data_ptr(),
-        int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0), native.ptr(weights), loss.data_ptr(),
-        native.ptr(stats), T, V, ids.shape[1], 1.0 / temperature, x.element_size(),
-        grad.element_size() if grad is not None else x.element_size(), native.stream_of(x.device)), "distill_row")
+    loss = x.new_empty(T, dtype=torch.float32)
+    size = x.element_size()
+    gp, gld, gsize = (None, 0, size) if grad is None else (grad.data_ptr(), grad.stride(0), grad.element_size())
+    rc = native.launch(
+        native.load().stb_distill_row, x.get_device(), x.data_ptr(), x.stride(0), gp, gld, ids.data_ptr(),
+        int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0),
+        None if weights is None else weights.data_ptr(), loss.data_ptr(), None if stats is None else stats.data_ptr(), T, V,
+        ids.shape[1], 1.0 / temperature, size, gsize, native.status_ptr(x.get_device()))
+    if rc:
+        native.check(rc, f"distill_row T={T} V={V} K={ids.shape[1]}")
     count_launch()
     return loss
 
@@ -137,21 +155,21 @@ def _row_kernel(x, ids, t, temperature, weights=None, grad=None, stats=None):
 def _stats_kernels(x, ids, t, temperature, vocab_start=0, group=None):
     """``(loss, statistics)`` of rows of any length, or of the shards of a group."""
     T, V = x.shape
-    K, vocab = ids.shape[1], V * _group_size(group)
-    lib, st = native.load(), native.stream_of(x.device)
-    stats = torch.empty((T, 4), dtype=torch.float32, device=x.device)
-    picked = torch.empty((T, K), dtype=torch.float32, device=x.device)
-    native.check(lib.stb_distill_stats(
-        x.data_ptr(), x.stride(0), ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(),
-        t.stride(0), stats.data_ptr(), picked.data_ptr(), T, V, K, vocab_start, vocab, 1.0 / temperature,
-        x.element_size(), st), "distill_stats")
+    K, vocab, index = ids.shape[1], V * _group_size(group), x.get_device()
+    lib = native.load()
+    stats = x.new_empty((T, 4), dtype=torch.float32)
+    picked = x.new_empty((T, K), dtype=torch.float32)
+    native.check(native.launch(
+        lib.stb_distill_stats, index, x.data_ptr(), x.stride(0), ids.data_ptr(), int(ids.dtype == torch.int64),
+        ids.stride(0), t.data_ptr(), t.stride(0), stats.data_ptr(), picked.data_ptr(), T, V, K, vocab_start, vocab,
+        1.0 / temperature, x.element_size()), f"distill_stats T={T} V={V} K={K}")
     count_launch()
     if _group_size(group) > 1:
         _join_shards(stats, picked, group)
-    loss = torch.empty(T, dtype=torch.float32, device=x.device)
-    native.check(lib.stb_distill_loss(
-        ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0), stats.data_ptr(),
-        picked.data_ptr(), loss.data_ptr(), T, K, vocab, 1.0 / temperature, st), "distill_loss")
+    loss = x.new_empty(T, dtype=torch.float32)
+    native.check(native.launch(
+        lib.stb_distill_loss, index, ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0),
+        stats.data_ptr(), picked.data_ptr(), loss.data_ptr(), T, K, vocab, 1.0 / temperature), "distill_loss")
     count_launch()
     return loss, stats
 
@@ -169,19 +187,26 @@ def _join_shards(stats, picked, group) -> None:
 
 def _grad_kernel(x, ids, t, temperature, weights, stats, grad, vocab_start=0, vocab=None):
     T, V = x.shape
-    native.check(native.load().stb_distill_grad(
-        x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0), ids.data_ptr(), int(ids.dtype == torch.int64),
-        ids.stride(0), t.data_ptr(), t.stride(0), native.ptr(weights), stats.data_ptr(), T, V, ids.shape[1], vocab_start,
-        V if vocab is None else vocab, 1.0 / temperature, x.element_size(), grad.element_size(),
-        native.stream_of(x.device)), "distill_grad")
+    rc = native.launch(
+        native.load().stb_distill_grad, x.get_device(), x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0),
+        ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0), weights.data_ptr(),
+        stats.data_ptr(), T, V, ids.shape[1], vocab_start, V if vocab is None else vocab, 1.0 / temperature,
+        x.element_size(), grad.element_size())
+    if rc:
+        native.check(rc, f"distill_grad T={T} V={V} K={ids.shape[1]}")
     count_launch()
+
+
+def _whole_rows(x, vocab_start: int, group) -> bool:
+    """Whether the one-pass kernel takes these rows: the whole vocabulary, in the shared memory of a cluster."""
+    return vocab_start == 0 and (group is None or _group_size(group) == 1) and _fits_row(x.shape[1], x.element_size())
 
 
 def _loss_and_grad(x, ids, t, temperature, weights, grad, vocab_start=0, group=None):
     """Loss of the rows of ``x``, their weighted gradient into ``grad`` (which may be ``x``)."""
     if x.shape[0] == 0:
         return torch.empty(0, dtype=torch.float32, device=x.device)
-    if _group_size(group) == 1 and vocab_start == 0 and _fits_row(x.shape[1], x.element_size()):
+    if _whole_rows(x, vocab_start, group):
         return _row_kernel(x, ids, t, temperature, weights, grad)
     loss, stats = _stats_kernels(x, ids, t, temperature, vocab_start, group)
     _grad_kernel(x, ids, t, temperature, weights, stats, grad, vocab_start, x.shape[1] * _group_size(group))
@@ -201,15 +226,14 @@ class _TopkDistillationFn(torch.autograd.Function):
             loss = torch.empty(0, dtype=torch.float32, device=x.device)
             ctx.save_for_backward(x, ids, t, loss)
         else:
-            with native.on_device(x.device):
-                if _group_size(group) == 1 and vocab_start == 0 and _fits_row(x.shape[1], x.element_size()):
-                    stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device)
-                    loss = _row_kernel(x, ids, t, temperature, stats=stats)
-                else:
-                    loss, stats = _stats_kernels(x, ids, t, temperature, vocab_start, group)
+            if _whole_rows(x, vocab_start, group):
+                stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
+                loss = _row_kernel(x, ids, t, temperature, stats=stats)
+            else:
+                loss, stats = _stats_kernels(x, ids, t, temperature, vocab_start, group)
             ctx.save_for_backward(x, ids, t, stats)
         ctx.shape, ctx.dtype = logits.shape, logits.dtype
-        return loss.view(logits.shape[:-1])
+        return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])
 
     @staticmethod
     @once_differentiable
@@ -222,8 +246,7 @@ class _TopkDistillationFn(torch.autograd.Function):
         x, ids, t, stats = ctx.saved_tensors
         grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         if x.shape[0]:
-            with native.on_device(x.device):
-                _grad_kernel(x, ids, t, temperature, w, stats, grad, vocab_start, x.shape[1] * _group_size(group))
+            _grad_kernel(x, ids, t, temperature, w, stats, grad, vocab_start, x.shape[1] * _group_size(group))
         return grad.view(ctx.shape), None, None, None, None, None
 
 
@@ -234,7 +257,7 @@ def topk_distillation(logits, teacher_ids, teacher_logits, temperature: float = 
     ``teacher_ids`` are always ids of the whole vocabulary.  Differentiable with respect to ``logits``."""
     temperature = float(temperature)
     rows = math.prod(logits.shape[:-1])
-    ids, t = _checked(rows, logits.device, teacher_ids, teacher_logits, temperature, "topk_distillation")
+    ids, t = _checked(rows, logits.get_device(), teacher_ids, teacher_logits, temperature, "topk_distillation")
     return _TopkDistillationFn.apply(logits, ids, t, temperature, int(vocab_start), group)
 
 
@@ -257,11 +280,13 @@ def topk_distillation_loss_and_grad(logits, teacher_ids, teacher_logits, weights
     temperature = float(temperature)
     if logits.dim() != 2:
         raise ValueError(f"{what}: logits are [T, V], got {tuple(logits.shape)}")
-    x = _rows_of(logits.detach(), what)
-    ids, t = _checked(x.shape[0], x.device, teacher_ids, teacher_logits, temperature, what)
-    w = _token_weights(weights, x.shape[0], x.device, what)
+    x, index = _rows_of(logits.detach() if logits.requires_grad else logits, what), logits.get_device()
+    ids, t = _checked(x.shape[0], index, teacher_ids, teacher_logits, temperature, what)
+    w = _token_weights(weights, x.shape[0], index, what)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
+        if index >= 0:
+            return _loss_and_grad(x, ids, t, temperature, w, out), out
     else:
         if out.shape != x.shape or out.device != x.device:
             raise ValueError(f"{what}: out is {tuple(out.shape)} on {out.device}, logits {tuple(x.shape)} on {x.device}")
@@ -281,8 +306,7 @@ def topk_distillation_loss_and_grad(logits, teacher_ids, teacher_logits, weights
         with torch.no_grad():
             out.copy_(_weighted(grad, w).to(out.dtype))
         return loss, out
-    with native.on_device(x.device):
-        loss = _loss_and_grad(x, ids, t, temperature, w, out)
+    loss = _loss_and_grad(x, ids, t, temperature, w, out)
     torch.autograd.graph.increment_version(out)
     return loss, out
 
@@ -300,33 +324,32 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
         dev = h.device
         need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         main_grad = getattr(w, "main_grad", None) if need_dw else None
-        with native.on_device(dev):
-            loss = torch.empty(T, dtype=torch.float32, device=dev)
-            dh = torch.empty((T, H), dtype=torch.float32, device=dev) if need_dh else None
-            dw = main_grad
-            if need_dw and dw is None:
-                dw = torch.empty((V, H), dtype=torch.float32, device=dev) if T else torch.zeros(
-                    (V, H), dtype=torch.float32, device=dev)
-            rows = min(chunk, T)
-            logits = torch.empty((rows, V), dtype=torch.float32, device=dev)
-            grad = torch.empty((rows, V), dtype=torch.bfloat16, device=dev) if need_dh or need_dw else None
-            for t0 in range(0, T, chunk):
-                n = min(T - t0, chunk)
-                s, hc = logits[:n], h[t0:t0 + n]
-                gemm(hc, w, out=s)
-                args = (s, ids[t0:t0 + n], t[t0:t0 + n], temperature)
-                if grad is None:
-                    if _group_size(group) == 1 and vocab_start == 0 and _fits_row(V, 4):
-                        loss[t0:t0 + n] = _row_kernel(*args)
-                    else:
-                        loss[t0:t0 + n] = _stats_kernels(*args, vocab_start, group)[0]
-                    continue
-                g = grad[:n]
-                loss[t0:t0 + n] = _loss_and_grad(*args, weights[t0:t0 + n], g, vocab_start, group)
-                if need_dh:
-                    gemm(g, w, b_mn_major=True, out=dh[t0:t0 + n])
-                if need_dw:
-                    gemm(g, hc, a_mn_major=True, b_mn_major=True, out=dw, accumulate=main_grad is not None or t0 > 0)
+        loss = torch.empty(T, dtype=torch.float32, device=dev)
+        dh = torch.empty((T, H), dtype=torch.float32, device=dev) if need_dh else None
+        dw = main_grad
+        if need_dw and dw is None:
+            dw = torch.empty((V, H), dtype=torch.float32, device=dev) if T else torch.zeros(
+                (V, H), dtype=torch.float32, device=dev)
+        rows = min(chunk, T)
+        logits = torch.empty((rows, V), dtype=torch.float32, device=dev)
+        grad = torch.empty((rows, V), dtype=torch.bfloat16, device=dev) if need_dh or need_dw else None
+        for t0 in range(0, T, chunk):
+            n = min(T - t0, chunk)
+            s, hc = logits[:n], h[t0:t0 + n]
+            gemm(hc, w, out=s)
+            args = (s, ids[t0:t0 + n], t[t0:t0 + n], temperature)
+            if grad is None:
+                if _whole_rows(s, vocab_start, group):
+                    loss[t0:t0 + n] = _row_kernel(*args)
+                else:
+                    loss[t0:t0 + n] = _stats_kernels(*args, vocab_start, group)[0]
+                continue
+            g = grad[:n]
+            loss[t0:t0 + n] = _loss_and_grad(*args, weights[t0:t0 + n], g, vocab_start, group)
+            if need_dh:
+                gemm(g, w, b_mn_major=True, out=dh[t0:t0 + n])
+            if need_dw:
+                gemm(g, hc, a_mn_major=True, b_mn_major=True, out=dw, accumulate=main_grad is not None or t0 > 0)
         ctx.save_for_backward(dh)
         ctx.dw = None if main_grad is not None else dw
         ctx.w_ref = w
@@ -367,13 +390,15 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
         raise ValueError(f"{what}: chunk_tokens must be positive, got {chunk_tokens}")
     if w.device != h.device:
         raise ValueError(f"{what}: h on {h.device}, w on {w.device}")
-    ids, t = _checked(h.shape[0], h.device, teacher_ids, teacher_logits, temperature, what)
-    wt = _token_weights(weights, h.shape[0], h.device, what)
+    ids, t = _checked(h.shape[0], h.get_device(), teacher_ids, teacher_logits, temperature, what)
+    wt = _token_weights(weights, h.shape[0], h.get_device(), what)
     if not h.is_cuda:
         loss = topk_distillation(torch.nn.functional.linear(h, w), ids, t, temperature, vocab_start, group)
         return torch.where(wt == 0, 0.0, loss * wt).sum(), loss.detach()
     if h.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise TypeError(f"{what}: h and w are bf16, got {h.dtype} and {w.dtype}")
+    if h.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{what}: h is on {h.device}, which is not the current device (the GEMMs go to the current one)")
     if w.shape[0] % 8 or w.shape[1] % 8 or w.data_ptr() % 16 or w.stride(1) != 1 or w.stride(0) % 8:
         raise ValueError(f"{what}: w needs a vocabulary and a hidden size that are multiples of 8 and 16-byte aligned "
                          f"rows, got {tuple(w.shape)} with strides {w.stride()}")

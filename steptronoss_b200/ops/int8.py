@@ -25,18 +25,21 @@ native.register_signature("stb_norm_quant", [P, P, P, P, P, P, L, I, L, L, L, L,
 
 
 def _no_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient: run frozen models under torch.no_grad() or detach the operands")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: run frozen models under torch.no_grad() or detach the operands")
 
 
-def pitched_int8(rows: int, width: int, device) -> torch.Tensor:
-    """An uninitialised int8 ``[rows, width]`` whose rows start on 16-byte boundaries."""
-    return torch.empty((rows, (width + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :width]
+def pitched_int8(rows: int, width: int, like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised int8 ``[rows, width]`` on the device of ``like`` whose rows start on 16-byte boundaries."""
+    q = like.new_empty((rows, (width + 15) // 16 * 16), dtype=torch.int8)
+    return q if width % 16 == 0 else q[:, :width]
 
 
 def pitched_like(q: torch.Tensor) -> torch.Tensor:
     """A copy of int8 rows with a pitch that the product takes."""
-    out = pitched_int8(q.shape[0], q.shape[1], q.device)
+    out = pitched_int8(q.shape[0], q.shape[1], q)
     out.copy_(q)
     return out
 
@@ -69,13 +72,13 @@ def quantize_rows_int8(x: torch.Tensor):
         raise ValueError(f"quantize_rows_int8 takes rows of at most {MAX_ROW} columns, got {K}")
     if x.stride(1) != 1 and K > 1:
         x = x.contiguous()
-    q = pitched_int8(M, K, x.device)
-    s = torch.empty(M, dtype=torch.float32, device=x.device)
+    q = pitched_int8(M, K, x)
+    s = x.new_empty(M, dtype=torch.float32)
     if M:
-        with native.on_device(x.device):
-            rc = native.load().stb_norm_quant(x.data_ptr(), None, None, None, q.data_ptr(), s.data_ptr(), M, K, x.stride(0),
-                                              0, 0, q.stride(0), 0.0, 0, 0, native.stream_of(x.device))
-        native.check(rc, f"quantize_rows_int8 M={M} K={K}")
+        rc = native.launch(native.load().stb_norm_quant, x.get_device(), x.data_ptr(), None, None, None, q.data_ptr(),
+                           s.data_ptr(), M, K, x.stride(0), 0, 0, q.stride(0), 0.0, 0, 0)
+        if rc:
+            native.check(rc, f"quantize_rows_int8 M={M} K={K}")
         count_launch()
     return q, s
 
@@ -92,8 +95,9 @@ def gemm_int8_reference(xq, sx, wq, sw, out_dtype: torch.dtype = torch.bfloat16)
 
 
 def _rows_aligned(t: torch.Tensor) -> bool:
-    return t.data_ptr() % 16 == 0 and (t.shape[1] == 1 or t.stride(1) == 1) and (
-        t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])
+    pitch, step = t.stride()
+    rows, width = t.shape
+    return t.data_ptr() % 16 == 0 and pitch % 16 == 0 and pitch >= width and (step == 1 or width == 1) or rows == 0
 
 
 def gemm_int8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor,
@@ -110,37 +114,43 @@ def gemm_int8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
     if sx.dtype != torch.float32 or sw.dtype != torch.float32 or sx.shape != (M,) or sw.shape != (N,):
         raise ValueError(f"gemm_int8 takes fp32 scales [{M}] and [{N}], got {sx.dtype} {tuple(sx.shape)} and "
                          f"{sw.dtype} {tuple(sw.shape)}")
-    if any(t.device != xq.device for t in (sx, wq, sw)):
+    index = xq.get_device()              # -1 on the CPU
+    if wq.get_device() != index or sx.get_device() != index or sw.get_device() != index:
         raise ValueError("gemm_int8: operands on different devices")
     if not 1 <= K <= MAX_K:
         raise ValueError(f"gemm_int8 takes 1 <= K <= {MAX_K}, got {K}")
     if out is not None:
         out_dtype = out.dtype
-        if out.shape != (M, N) or out.device != xq.device or (N > 1 and out.stride(1) != 1) or (
+        if out.shape != (M, N) or out.get_device() != index or (N > 1 and out.stride(1) != 1) or (
                 M > 1 and out.stride(0) < N):
             raise ValueError(f"gemm_int8: out must be [{M}, {N}] on {xq.device} with separate rows and a contiguous last "
                              f"dimension, got {tuple(out.shape)} with strides {out.stride()} on {out.device}")
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    if out_dtype != torch.bfloat16 and out_dtype != torch.float32:
         raise TypeError(f"gemm_int8 writes bf16 or fp32, not {out_dtype}")
     _no_gradient("gemm_int8", sx, sw, out)
-    if not xq.is_cuda:
+    if index < 0:
         res = gemm_int8_reference(xq, sx, wq, sw, out_dtype)
         return res if out is None else out.copy_(res)
-    for name, t in (("xq", xq), ("wq", wq)):
-        if t.shape[0] and not _rows_aligned(t):
-            raise ValueError(f"gemm_int8: rows of {name} must start on 16-byte boundaries and be contiguous, got strides "
-                             f"{t.stride()} (quantize_rows_int8 returns such rows, pitched_like makes them)")
+    if not _rows_aligned(xq) or not _rows_aligned(wq):
+        raise ValueError(f"gemm_int8: the rows of xq and wq must be contiguous and start on 16-byte boundaries, got "
+                         f"strides {xq.stride()} and {wq.stride()} (quantize_rows_int8 returns such rows, pitched_like "
+                         "makes them)")
+    given = out
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=xq.device)
+        out = xq.new_empty((M, N), dtype=out_dtype)
     if M and N:
-        sx, sw = sx.contiguous(), sw.contiguous()
-        with native.on_device(xq.device):
-            rc = native.load().stb_gemm_int8(
-                xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, xq.stride(0),
-                wq.stride(0), out.stride(0) if M > 1 else max(out.stride(0), N), int(out_dtype == torch.float32),
-                native.status_word(xq.device).data_ptr(), native.stream_of(xq.device))
-        native.check(rc, f"gemm_int8 M={M} N={N} K={K}")
+        if not sx.is_contiguous():
+            sx = sx.contiguous()
+        if not sw.is_contiguous():
+            sw = sw.contiguous()
+        rc = native.launch(native.load().stb_gemm_int8, index, xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(),
+                           out.data_ptr(), M, N, K, xq.stride(0), wq.stride(0), out.stride(0) if M > 1 else N,
+                           int(out_dtype == torch.float32), native.status_ptr(index))
+        if rc:
+            native.check(rc, f"gemm_int8 M={M} N={N} K={K}")
         count_launch()
+        if given is not None:
+            torch.autograd.graph.increment_version(out)
     return out
 
 
@@ -149,6 +159,6 @@ def linear_int8(x: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, out_dtype: 
     _no_gradient("linear_int8", x, sw)
     if x.dim() < 1 or wq.dim() != 2 or x.shape[-1] != wq.shape[1]:
         raise ValueError(f"linear_int8 takes [..., K] and [N, K], got {tuple(x.shape)} and {tuple(wq.shape)}")
-    q, s = quantize_rows_int8(x.reshape(-1, x.shape[-1]))
+    q, s = quantize_rows_int8(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
     y = gemm_int8(q, s, wq, sw, out_dtype=out_dtype or torch.bfloat16)
-    return y.view(*x.shape[:-1], wq.shape[0])
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], wq.shape[0])

@@ -47,41 +47,48 @@ def _run(x, delta, weight, eps, zero_centered, fmt, what):
         raise ValueError(f"{what}: weight {tuple(weight.shape)} does not fit rows of {tuple(x.shape)}")
     if delta is not None and delta.shape != x.shape:
         raise ValueError(f"{what}: x {tuple(x.shape)} and delta {tuple(delta.shape)} differ")
-    if any(t is not None and t.device != x.device for t in (delta, weight)):
+    index = x.get_device()              # -1 on the CPU
+    if weight.get_device() != index or (delta is not None and delta.get_device() != index):
         raise ValueError(f"{what}: operands on different devices")
     H = x.shape[-1]
     if fmt == "e4m3_1x128" and H % 128:
         raise ValueError(f"{what}: e4m3 blocks need a multiple of 128 columns, got {H}")
     _no_gradient(what, x, delta, weight)
-    x2 = x.reshape(-1, H)
-    d2 = delta.reshape(-1, H) if delta is not None else None
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, H)
+    d2 = delta if flat or delta is None else delta.reshape(-1, H)
     rows = x2.shape[0]
-    if not x.is_cuda:
+    if index < 0:
         s = x2 if d2 is None else (x2.float() + d2.float()).to(x.dtype)
         q, scale = _statement(s, weight, eps, zero_centered, fmt)
         return s, q, scale
-    if any(t is not None and t.dtype != torch.bfloat16 for t in (x, delta, weight)):
+    bf16 = torch.bfloat16
+    if x.dtype != bf16 or weight.dtype != bf16 or (delta is not None and delta.dtype != bf16):
         raise TypeError(f"{what}: x, delta and weight are bf16 on the GPU")
     if H > MAX_ROW:
         raise ValueError(f"{what}: at most {MAX_ROW} columns, got {H}")
-    x2 = x2 if x2.stride(1) == 1 else x2.contiguous()
-    if d2 is not None and d2.stride(1) != 1:
-        d2 = d2.contiguous()
-    weight = weight.contiguous()
-    s = torch.empty((rows, H), dtype=torch.bfloat16, device=x.device) if d2 is not None else None
+    if x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    s, sp, dp, ldd = None, None, None, 0
+    if d2 is not None:
+        if d2.stride(1) != 1:
+            d2 = d2.contiguous()
+        s = x2.new_empty((rows, H))
+        sp, dp, ldd = s.data_ptr(), d2.data_ptr(), d2.stride(0)
+    if weight.stride(0) != 1:
+        weight = weight.contiguous()
     if fmt == "int8":
-        q = pitched_int8(rows, H, x.device)
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        q = pitched_int8(rows, H, x2)
+        scale = x2.new_empty(rows, dtype=torch.float32)
     else:
-        q = torch.empty((rows, H), dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty((rows, H // 128), dtype=torch.float32, device=x.device)
+        q = x2.new_empty((rows, H), dtype=torch.float8_e4m3fn)
+        scale = x2.new_empty((rows, H // 128), dtype=torch.float32)
     if rows:
-        with native.on_device(x.device):
-            rc = native.load().stb_norm_quant(
-                x2.data_ptr(), native.ptr(d2), weight.data_ptr(), native.ptr(s), q.data_ptr(), scale.data_ptr(), rows, H,
-                x2.stride(0), d2.stride(0) if d2 is not None else 0, H, q.stride(0), float(eps), int(zero_centered),
-                FORMATS.index(fmt), native.stream_of(x.device))
-        native.check(rc, f"{what} rows={rows} H={H} {fmt}")
+        rc = native.launch(native.load().stb_norm_quant, index, x2.data_ptr(), dp, weight.data_ptr(), sp, q.data_ptr(),
+                           scale.data_ptr(), rows, H, x2.stride(0), ldd, H, q.stride(0), eps, int(zero_centered),
+                           int(fmt != "int8"))
+        if rc:
+            native.check(rc, f"{what} rows={rows} H={H} {fmt}")
         count_launch()
     return s, q, scale
 
@@ -95,4 +102,4 @@ def rmsnorm_quant(x, weight, eps: float = 1e-6, zero_centered: bool = False, fmt
 def add_rmsnorm_quant(x, delta, weight, eps: float = 1e-6, zero_centered: bool = False, fmt: str = "int8"):
     """``(x + delta, q, scales)``: the residual stream and ``rmsnorm`` of it in 8 bits (``q [rows, H]``)."""
     s, q, scale = _run(x, delta, weight, eps, zero_centered, fmt, "add_rmsnorm_quant")
-    return s.view(x.shape), q, scale
+    return s if x.dim() == 2 else s.view(x.shape), q, scale

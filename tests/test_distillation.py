@@ -382,7 +382,7 @@ def test_strides_alignment_and_in_place(dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 330001), (torch.float32, 163900)])
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 600001), (torch.float32, 300001)])
 def test_rows_longer_than_a_cluster_holds(dtype, V):
     from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
     from steptronoss_b200.ops.distillation import _fits_row
@@ -392,10 +392,10 @@ def test_rows_longer_than_a_cluster_holds(dtype, V):
     ids[0, 3] = ids[0, 2]
     loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w, 0.7)
     # this kernel adds V / 512 exponentials per thread: a longer chain than the bound's 200, of V / 512 + 16
-    assert V / 512 + 16 < 700
+    assert V / 512 + 16 < 1200
     want, wgrad, p, q = oracle(logits, ids, teacher, 0.7, weights=w)
     loss_tol, grad_tol = bounds(logits.cpu(), teacher.cpu(), 0.7, p, q, wgrad, w.double().cpu(), dtype)
-    more = 500 * 2.0 ** -24
+    more = 1000 * 2.0 ** -24
     assert (loss.double().cpu() - want).abs().max() <= loss_tol + more
     assert ((grad.double().cpu() - wgrad).abs() <= grad_tol + w.double().cpu()[:, None] / 0.7 * p * more).all()
     buf = logits.clone()
@@ -431,7 +431,7 @@ def test_shards_joined_by_hand_equal_the_whole(dtype):
     teacher[1] = -INF
     logits[2, :1000] = -INF                        # one shard without any probability
     ids[2] = torch.arange(1500, 1500 + K, device="cuda")
-    lib, st = native.load(), native.stream_of(logits.device)
+    lib, st = native.load(), native.stream()
     stats, picked = [], []
     for r in range(parts):
         x = logits[:, r * 1000:(r + 1) * 1000]
@@ -480,7 +480,7 @@ def test_fused_head_follows_the_definition(T, H, V, chunk):
     e = H * 2.0 ** -24 * mag / tau
     loss_tol, _ = bounds(logits.cpu(), teacher.cpu(), tau, p, q, g, w.double().cpu(), torch.bfloat16)
     assert (tok.double().cpu() - want).abs().max() <= loss_tol + 2 * e
-    assert abs(float(total) - float((want * w.double().cpu()).sum())) <= (loss_tol + 2 * e) * float(w.sum()) * 1.01
+    assert abs(float(total.detach()) - float((want * w.double().cpu()).sum())) <= (loss_tol + 2 * e) * float(w.sum()) * 1.01
     # gradient rows are rounded to bf16 (2^-8 of each), the products summed in fp32 and rounded once more
     for got, a, b in ((dh, g, head.detach().double().cpu()), (dw, g.t(), h.detach().double().cpu())):
         exact, size = a @ b, a.abs() @ b.abs()
