@@ -310,13 +310,79 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// Elements of granule g of the row: from the slice in shared memory, or one by one from the row at its two ends.
-template <typename T>
-__device__ __forceinline__ uint4 slice_granule(const uint4* slice, const T* row, int g, int g0, int lead, int V) {
-  constexpr int n = Lane<T>::n;
-  const int a = g * n - lead;
-  if (a >= 0 && a + n <= V) return slice[g - g0];
-  return load_granule<T>(row, g, lead, V);
+// Two fp32 at once: one instruction on this architecture.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t ex2_2(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  return pair(ex2(a), ex2(b));
+}
+
+// A granule as pairs, its largest value, and pairs back to an output granule.
+template <typename T> struct Pairs;
+template <> struct Pairs<__nv_bfloat16> {
+  static constexpr int n = 4;
+  static __device__ __forceinline__ void widen(const uint4& u, uint64_t (&f)[4]) {
+    f[0] = pair(bf16_lo(u.x), bf16_hi(u.x));
+    f[1] = pair(bf16_lo(u.y), bf16_hi(u.y));
+    f[2] = pair(bf16_lo(u.z), bf16_hi(u.z));
+    f[3] = pair(bf16_lo(u.w), bf16_hi(u.w));
+  }
+  static __device__ __forceinline__ float top(const uint4& u) {      // a NaN is passed over; the sum shows it
+    uint32_t m;
+    asm("{\n\t.reg .b32 a, b;\n\tmax.bf16x2 a, %1, %2;\n\tmax.bf16x2 b, %3, %4;\n\tmax.bf16x2 %0, a, b;\n\t}"
+        : "=r"(m) : "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w));
+    return fmaxf(bf16_lo(m), bf16_hi(m));
+  }
+};
+template <> struct Pairs<float> {
+  static constexpr int n = 2;
+  static __device__ __forceinline__ void widen(const uint4& u, uint64_t (&f)[2]) {
+    f[0] = pair(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = pair(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+};
+template <typename TO, int NP>
+__device__ __forceinline__ void store_pairs(TO* at, bool aligned, const uint64_t (&f)[NP]) {
+  float v[2 * NP];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) unpair(f[j], v[2 * j], v[2 * j + 1]);
+  if (aligned) {
+    if constexpr (sizeof(TO) == 4) {
+      *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if constexpr (NP == 4) {
+      *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                                                 pack_bf16(v[6], v[7]));
+    } else {
+      *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2 * NP; ++j) Lane<TO>::store(at + j, v[j]);
+  }
 }
 
 template <typename T, typename TO, int C>
@@ -494,44 +560,62 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
       };
       const T* src = static_cast<const T*>(p.logits) + row * p.ld;
       const Granules<T> gr(src, p.V);
-      const int g0 = rank * plan.per, g1 = min(g0 + plan.per, gr.count);
-      const uint4* slice = reinterpret_cast<const uint4*>(dyn + slot * slice_bytes);
+      // granules [gs, ge) of the slice are whole; the row's elements before the first and behind the last whole granule
+      // (fewer than n each) go to a thread of their own
+      const int g0 = rank * plan.per, whole = (gr.lead + p.V) / n;
+      const int gs = max(g0, gr.lead > 0 ? 1 : 0), ge = min(g0 + plan.per, whole);
+      const uint4* slice = reinterpret_cast<const uint4*>(dyn + slot * slice_bytes) - g0;
+      int edge = -1;
+      if (threadIdx.x < 8) {
+        if (rank == 0 && gr.lead > 0 && static_cast<int>(threadIdx.x) < min(n - gr.lead, p.V)) edge = threadIdx.x;
+      } else if (threadIdx.x < 16) {
+        const int at = whole * n - gr.lead + static_cast<int>(threadIdx.x) - 8;
+        if (whole >= g0 && whole < g0 + plan.per && (whole > 0 || gr.lead == 0) && at < p.V) edge = at;
+      }
+      const float x_edge = edge >= 0 ? Lane<T>::value(src + edge) : 0.f;
       wait(&bars.full[slot], (it / plan.slots) & 1);
       // pass 1: a thread that has seen nothing but -inf adds exp2(-inf) = 0
-      constexpr int kU = 4;
-      float top = -INFINITY, sums[kU];
-#pragma unroll
-      for (int u = 0; u < kU; ++u) sums[u] = 0.f;
-      for (int g = g0 + threadIdx.x; g < g1; g += kRowCompute * kU) {
-        uint4 v[kU];
+      constexpr int kU = 4, kP = Pairs<T>::n;
+      const uint64_t c2 = pair(c, c);
+      float top = edge >= 0 ? x_edge * c : -INFINITY;
+      uint64_t acc[2] = {0, 0};                       // two pairs of sums
+      if (edge >= 0) acc[0] = pair(ex2(x_edge * c - (top == -INFINITY ? 0.f : top)), 0.f);
+      if (top != top) top = -INFINITY;
+      auto take = [&](const uint4* v, int count) {
         float m = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          if (g + u * kRowCompute >= g1) continue;
-          v[u] = slice_granule<T>(slice, src, g + u * kRowCompute, g0, gr.lead, p.V);
-          float f[n];
-          Lane<T>::widen(v[u], f);
-#pragma unroll
-          for (int j = 0; j < n; ++j) m = fmaxf(m, f[j]);
-        }
+        for (int u = 0; u < count; ++u) m = fmaxf(m, Pairs<T>::top(v[u]));
         m *= c;
         if (m > top) {
           const float scale = ex2(top - m);
-#pragma unroll
-          for (int u = 0; u < kU; ++u) sums[u] *= scale;
+          acc[0] = mul2(acc[0], pair(scale, scale));
+          acc[1] = mul2(acc[1], pair(scale, scale));
           top = m;
         }
         const float base = top == -INFINITY ? 0.f : top;
+        const uint64_t minus = pair(-base, -base);
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          if (g + u * kRowCompute >= g1) continue;
-          float f[n];
-          Lane<T>::widen(v[u], f);
+        for (int u = 0; u < count; ++u) {
+          uint64_t f[kP];
+          Pairs<T>::widen(v[u], f);
 #pragma unroll
-          for (int j = 0; j < n; ++j) sums[u] += ex2(fmaf(f[j], c, -base));
+          for (int j = 0; j < kP; ++j) acc[j & 1] = add2(acc[j & 1], ex2_2(fma2(f[j], c2, minus)));
         }
+      };
+      int g = gs + static_cast<int>(threadIdx.x);
+      for (; g + (kU - 1) * kRowCompute < ge; g += kU * kRowCompute) {
+        uint4 v[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) v[u] = slice[g + u * kRowCompute];
+        take(v, kU);
       }
-      float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      for (; g < ge; g += kRowCompute) {
+        const uint4 v = slice[g];
+        take(&v, 1);
+      }
+      float sum, sum1;
+      unpair(add2(acc[0], acc[1]), sum, sum1);
+      sum += sum1;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1)
         merge(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
@@ -576,15 +660,22 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         const float w = p.weight != nullptr ? p.weight[row] : 1.f;
         // no entries, or a token that does not count: zero whatever the logits hold
         const bool zero = head[b].tsum == 0.f || w == 0.f;
-        const float inv = __fdiv_rn(1.f, sum), gw = w * p.inv_tau, gs = gw * inv;
+        const float inv = __fdiv_rn(1.f, sum), gw = w * p.inv_tau, scale = gw * inv;
+        const uint64_t scale2 = pair(scale, scale), minus = pair(-top, -top);
+        TO* at = dst - gr.lead;
 #pragma unroll kU
-        for (int g = g0 + threadIdx.x; g < g1; g += kRowCompute) {
-          float f[n];
-          Lane<T>::widen(slice_granule<T>(slice, src, g, g0, gr.lead, p.V), f);
+        for (int k = gs + static_cast<int>(threadIdx.x); k < ge; k += kRowCompute) {
+          uint64_t f[kP];
+          Pairs<T>::widen(slice[k], f);
 #pragma unroll
-          for (int j = 0; j < n; ++j) f[j] = zero ? 0.f : ex2(fmaf(f[j], c, -top)) * gs;
-          store_granule<TO, n>(dst, g, gr.lead, p.V, aligned, f);
+          for (int j = 0; j < kP; ++j) f[j] = mul2(ex2_2(fma2(f[j], c2, minus)), scale2);
+          if (zero) {
+#pragma unroll
+            for (int j = 0; j < kP; ++j) f[j] = 0;
+          }
+          store_pairs<TO, kP>(at + k * n, aligned, f);
         }
+        if (edge >= 0) Lane<TO>::store(dst + edge, zero ? 0.f : ex2(fmaf(x_edge, c, -top)) * scale);
         mbar_arrive_warp(&bars.empty[slot]);
         compute_barrier();                 // the dense gradient is written
         if (!zero) {
