@@ -149,6 +149,20 @@ __device__ __forceinline__ void merge(float& m, float& s, float om, float os) {
   s = a + b;
 }
 
+// The same over the lanes of a warp: the largest top first, then one scaling and a plain sum.
+__device__ __forceinline__ float warp_top(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ void warp_merge(float& m, float& s) {
+  const float top = warp_top(m);
+  if (m != top) s *= ex2(m - top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  m = top;
+}
+
 // Teacher entries of a row in shared memory, filled by warp 0.
 struct Entries {
   float q[kDsMaxEntries];      // probability, 0 where there is no entry
@@ -261,36 +275,40 @@ __device__ __forceinline__ void block_merge(float& m, float& s, float2* red) {
 // Persistent clusters of C CTAs; a cluster takes every (number of clusters)-th row and each of its CTAs a contiguous
 // slice of the row's granules, which stays in shared memory between the two passes over it:
 //
-//   producer warp   bulk copies of the slices of coming rows into a ring of `slots` buffers
-//   entries warp    the teacher's entries one row ahead: their statistics, and the list of those that fall into this
-//                   CTA's slice
-//   compute warps   pass 1: (top, sum) of the slice; every CTA sends its pair to all CTAs of the cluster (st.async onto
-//                   their mbarriers); pass 2: the gradient from the same shared memory, straight to global memory; then
-//                   the gradient at the entries once more, with q
+//   producer warp   bulk copies of 16 KB chunks into a ring that runs on from row to row: a chunk that pass 2 has read is
+//                   filled with the next row's logits at once
+//   entries warps   two, for even and odd rows: the teacher's entries of a coming row, their statistics and the list of
+//                   those that fall into this CTA's slice; behind pass 2 the loss and the gradient at the entries
+//   compute warps   pass 1: (top, sum) of the slice.  Every warp sends its pair to all CTAs of the cluster (st.async onto
+//                   their mbarriers) and merges all pairs when they are there.  Pass 2: the gradient from the same shared
+//                   memory, straight to global memory
 //
-// The copies run ahead of the arithmetic, so DRAM is busy while a CTA waits for its cluster's sums.  Measured before
-// with the row in registers and one cluster per row: 2.2 TB/s for 4096 rows of 151936 bf16, the chain launch - load -
-// entries - exchange - store exposed for every row.
-constexpr int kRowCompute = 256;
-constexpr int kRowThreads = kRowCompute + 64;
+// Loads, entries and the cluster's exchange thus run beside the arithmetic; nothing waits for the whole CTA.
+// Bound: DRAM for fp32 logits; for bf16 the exponentials (two per element, 16 a cycle and SM) come close to it.
+constexpr int kU = 4;                            // granules per compute thread and chunk
+constexpr int kRowWarps = 8;                     // compute warps
+constexpr int kRowCompute = 32 * kRowWarps;
+constexpr int kRowThreads = kRowCompute + 96;
+constexpr int kChunk = kRowCompute * kU;         // granules: 16 KB
+constexpr int kMaxChunks = 12;
 
 struct RowPlan {
   int per;             // granules per CTA
-  int slots;
+  int chunks;          // per slice
+  int ring;            // chunks in shared memory, at least those of a slice
   int clusters;
   int kpad;            // K rounded up to 4
 };
 struct RowBars {
-  uint64_t full[4], empty[4];       // slices
-  uint64_t e_full[2], e_empty[2];   // entries
+  uint64_t full[kMaxChunks], empty[kMaxChunks];
+  uint64_t e_full[2], e_empty[2];   // entries prepared; pass 2 of their row done
   uint64_t xchg[2];                 // the cluster's pairs
 };
 // Entries of a row, arrays of kpad: for the loss q, log2 q, s; of this CTA's slice q, s, the q of the gradient (summed
 // over equal ids, -1: another entry carries it), id.
 struct EntryHead {
-  float tmax, tsum;
-  int own;             // entries in this CTA's slice
-  int pad;
+  float tmax, tsum, weight;
+  float top, sum;      // of the row, from the compute warps
 };
 
 __host__ __device__ constexpr int entry_bytes(int kpad) { return kpad * 28; }
@@ -308,8 +326,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
 // Two fp32 at once: one instruction on this architecture.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -348,10 +364,15 @@ template <> struct Pairs<__nv_bfloat16> {
     f[2] = pair(bf16_lo(u.z), bf16_hi(u.z));
     f[3] = pair(bf16_lo(u.w), bf16_hi(u.w));
   }
-  static __device__ __forceinline__ float top(const uint4& u) {      // a NaN is passed over; the sum shows it
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     uint32_t m;
-    asm("{\n\t.reg .b32 a, b;\n\tmax.bf16x2 a, %1, %2;\n\tmax.bf16x2 b, %3, %4;\n\tmax.bf16x2 %0, a, b;\n\t}"
-        : "=r"(m) : "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    return m;
+  }
+  static __device__ __forceinline__ float top(const uint4 (&v)[kU]) {      // a NaN is passed over; the sum shows it
+    uint32_t m = max2(max2(v[0].x, v[0].y), max2(v[0].z, v[0].w));
+#pragma unroll
+    for (int u = 1; u < kU; ++u) m = max2(m, max2(max2(v[u].x, v[u].y), max2(v[u].z, v[u].w)));
     return fmaxf(bf16_lo(m), bf16_hi(m));
   }
 };
@@ -361,8 +382,13 @@ template <> struct Pairs<float> {
     f[0] = pair(__uint_as_float(u.x), __uint_as_float(u.y));
     f[1] = pair(__uint_as_float(u.z), __uint_as_float(u.w));
   }
-  static __device__ __forceinline__ float top(const uint4& u) {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  static __device__ __forceinline__ float top(const uint4 (&v)[kU]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[u].x), __uint_as_float(v[u].y)),
+                         fmaxf(__uint_as_float(v[u].z), __uint_as_float(v[u].w))));
+    return m;
   }
 };
 template <typename TO, int NP>
@@ -385,85 +411,123 @@ __device__ __forceinline__ void store_pairs(TO* at, bool aligned, const uint64_t
   }
 }
 
+// Bounded waits of this kernel.  `soon`: due within a microsecond, polled without looking at the clock first, whose
+// reading alone takes that long.  `idle`: the warps that run ahead sleep between polls; polling without a pause took
+// a third of the issue slots from the compute warps.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t phase) {
+  for (int i = 0; i < 1024; ++i)
+    if (mbar_try_wait(bar, phase)) return true;
+  return mbar_wait(bar, phase);
+}
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t phase, unsigned ns) {
+  if (mbar_try_wait(bar, phase)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 1; i < kSpinLimit; ++i) {
+    __nanosleep(ns);
+    if (mbar_try_wait(bar, phase)) return true;
+    if ((i & 255u) == 0 && global_timer_ns() - t0 > kWaitBudgetNs) return false;
+  }
+  return false;
+}
+
+// Where the granules of this CTA's slice of a row are: [gs, ge) are whole; the row's elements before its first and behind
+// its last whole granule (fewer than n each) are `edge` elements, one for a thread of its own each.
+template <typename T>
+struct Slice {
+  int g0, gs, ge, whole;
+  __device__ __forceinline__ Slice(const Granules<T>& gr, int rank, int per, int V) {
+    g0 = rank * per;
+    whole = (gr.lead + V) / Lane<T>::n;
+    gs = max(g0, gr.lead > 0 ? 1 : 0);
+    ge = min(g0 + per, whole);
+  }
+  __device__ __forceinline__ int edge(const Granules<T>& gr, int rank, int per, int V, int thread) const {
+    constexpr int n = Lane<T>::n;
+    if (thread < 8) return rank == 0 && gr.lead > 0 && thread < min(n - gr.lead, V) ? thread : -1;
+    if (thread >= 16) return -1;
+    const int at = whole * n - gr.lead + thread - 8;
+    return whole >= g0 && whole < g0 + per && (whole > 0 || gr.lead == 0) && at < V ? at : -1;
+  }
+};
+
 template <typename T, typename TO, int C>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 2)
 distill_row_kernel(const DistillParams p, const RowPlan plan) {
   constexpr int n = Lane<T>::n;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ RowBars bars;
-  __shared__ float2 red[2][kRowCompute / 32];
-  __shared__ float2 part[2][C];
+  __shared__ float2 part[2][C * kRowWarps];
   __shared__ EntryHead head[2];
-  __shared__ volatile int failed[2];       // by row parity, so that all compute threads leave after the same row
+  __shared__ volatile int failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = C > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int first_row = blockIdx.x / C;
-  const int slice_bytes = plan.per * 16;
-  uint8_t* entry_base = dyn + plan.slots * slice_bytes;
-  uint32_t* bitmap = reinterpret_cast<uint32_t*>(entry_base + 2 * entry_bytes(plan.kpad));
+  uint8_t* entry_base = dyn + plan.ring * kChunk * 16;
+  const float c = p.inv_tau * kLog2e;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < plan.ring; ++i) {
       mbar_init(&bars.full[i], 1);
-      mbar_init(&bars.empty[i], kRowCompute / 32);
+      mbar_init(&bars.empty[i], kRowWarps);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.e_full[i], 1);
-      mbar_init(&bars.e_empty[i], kRowCompute / 32);
+      mbar_init(&bars.e_empty[i], kRowWarps);
       mbar_init(&bars.xchg[i], 1);
     }
-    failed[0] = failed[1] = 0;
+    failed = 0;
     fence_barrier_init();
   }
-  for (int i = threadIdx.x; i < bitmap_bytes(plan.per, n) / 4; i += kRowThreads) bitmap[i] = 0;
+  {
+    uint32_t* bitmaps = reinterpret_cast<uint32_t*>(entry_base + 2 * entry_bytes(plan.kpad));
+    for (int i = threadIdx.x; i < 2 * bitmap_bytes(plan.per, n) / 4; i += kRowThreads) bitmaps[i] = 0;
+  }
   __syncthreads();
   if constexpr (C > 1) {                   // the other CTAs' barriers are initialised, too
     cluster_arrive();
     cluster_wait();
   }
 
-  const float c = p.inv_tau * kLog2e;
-  if (warp == kRowCompute / 32) {
+  if (warp == kRowWarps) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
-      int it = 0;
-      for (int row = first_row; row < p.T; row += plan.clusters, ++it) {
-        const int slot = it % plan.slots;
-        if (!mbar_wait(&bars.empty[slot], ((it / plan.slots) & 1) ^ 1)) {
-          report_error(p.status, kErrProducerWait);
-          break;
-        }
+      int slot = 0;
+      uint32_t lap = 0;                    // parity of the ring's passes
+      bool ok = true;
+      for (int row = first_row; row < p.T && ok; row += plan.clusters) {
         const T* src = static_cast<const T*>(p.logits) + row * p.ld;
         const Granules<T> gr(src, p.V);
-        const int g0 = rank * plan.per;
-        const int gs = max(g0, gr.lead > 0 ? 1 : 0), ge = min(g0 + plan.per, (gr.lead + p.V) / n);
-        if (ge > gs) {
-          const uint32_t bytes = static_cast<uint32_t>(ge - gs) * 16;
-          mbar_arrive_expect_tx(&bars.full[slot], bytes);
-          bulk_load(dyn + slot * slice_bytes + (gs - g0) * 16, src + (static_cast<long long>(gs) * n - gr.lead), bytes,
-                    &bars.full[slot]);
-        } else {
-          mbar_arrive(&bars.full[slot]);
+        const Slice<T> sl(gr, rank, plan.per, p.V);
+        for (int k = 0; k < plan.chunks; ++k) {
+          ok = !failed && mbar_wait_idle(&bars.empty[slot], lap ^ 1, 100);
+          if (!ok) { report_error(p.status, kErrProducerWait); failed = 1; break; }
+          const int k0 = sl.g0 + k * kChunk, a = max(k0, sl.gs), b = min(k0 + kChunk, sl.ge);
+          if (b > a) {
+            const uint32_t bytes = static_cast<uint32_t>(b - a) * 16;
+            mbar_arrive_expect_tx(&bars.full[slot], bytes);
+            bulk_load(dyn + (slot * kChunk + a - k0) * 16, src + (static_cast<long long>(a) * n - gr.lead), bytes,
+                      &bars.full[slot]);
+          } else {
+            mbar_arrive(&bars.full[slot]);
+          }
+          if (++slot == plan.ring) { slot = 0; lap ^= 1; }
         }
       }
     }
-  } else if (warp > kRowCompute / 32) {
-    // ---------------------------------------------------------------- entries, one row ahead
-    int it = 0;
-    for (int row = first_row; row < p.T; row += plan.clusters, ++it) {
-      const int b = it & 1;
-      bool ok = mbar_wait(&bars.e_empty[b], ((it >> 1) & 1) ^ 1);
-      if (!__all_sync(0xffffffffu, ok)) {
-        report_error(p.status, kErrProducerWait);
-        break;
-      }
-      float* eq = reinterpret_cast<float*>(entry_base + b * entry_bytes(plan.kpad));
-      float *elq = eq + plan.kpad, *es = elq + plan.kpad, *oq = es + plan.kpad, *os = oq + plan.kpad;
-      float* gq = os + plan.kpad;
-      int* oid = reinterpret_cast<int*>(gq + plan.kpad);
+  } else if (warp > kRowWarps) {
+    // ---------------------------------------------------------------- entries of every second row
+    const int b = warp - kRowWarps - 1;
+    float* eq = reinterpret_cast<float*>(entry_base + b * entry_bytes(plan.kpad));
+    float *elq = eq + plan.kpad, *es = elq + plan.kpad, *oq = es + plan.kpad, *os = oq + plan.kpad, *gq = os + plan.kpad;
+    int* oid = reinterpret_cast<int*>(gq + plan.kpad);
+    uint32_t* bitmap = reinterpret_cast<uint32_t*>(entry_base + 2 * entry_bytes(plan.kpad) + b * bitmap_bytes(plan.per, n));
+    EntryHead& hd = head[b];
+    uint32_t phase = 0;
+    for (long long row = first_row + static_cast<long long>(b) * plan.clusters; row < p.T; row += 2ll * plan.clusters, phase ^= 1) {
       const T* src = static_cast<const T*>(p.logits) + row * p.ld;
       const Granules<T> gr(src, p.V);
       const int e0 = rank * plan.per * n - gr.lead, e1 = e0 + plan.per * n;
+      const float w = p.weight != nullptr ? p.weight[row] : 1.f;
       float tmax = -INFINITY;
       bool bad = false;                    // fmaxf drops a NaN; it has to reach the loss
       int own = 0;
@@ -472,11 +536,15 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         float t[2], sv[2];
         bool here[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) id[u] = j0 + 32 * u + lane < p.K ? entry_id(p, row, j0 + 32 * u + lane) : -1;
+        for (int u = 0; u < 2; ++u) {
+          const int j = j0 + 32 * u + lane;
+          id[u] = j < p.K ? entry_id(p, row, j) : -1;
+          t[u] = j < p.K ? p.teacher[row * p.ld_t + j] : -INFINITY;
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const bool in = id[u] >= 0 && id[u] < p.V;
-          t[u] = in ? p.teacher[row * p.ld_t + j0 + 32 * u + lane] : -INFINITY;
+          const bool in = id[u] >= 0 && id[u] < p.V && t[u] != -INFINITY;
+          if (!in) t[u] = -INFINITY;
           here[u] = in && id[u] >= e0 && id[u] < e1;
           sv[u] = in && (here[u] || rank == 0) ? Lane<T>::value(src + id[u]) : 0.f;
         }
@@ -486,9 +554,8 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           if (j < p.K) { elq[j] = t[u]; es[j] = sv[u]; }
           tmax = fmaxf(tmax, t[u]);
           bad |= t[u] != t[u];
-          const bool mine = here[u] && t[u] != -INFINITY;
-          const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-          if (mine) {
+          const uint32_t votes = __ballot_sync(0xffffffffu, here[u]);
+          if (here[u]) {
             const int at = own + __popc(votes & ((1u << lane) - 1));
             oid[at] = static_cast<int>(id[u]);
             oq[at] = t[u];
@@ -508,12 +575,18 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         tsum += e;
       }
       tsum = warp_total(tsum);
+      // what the compute warps need, and the word that the logits at the entries have been read
+      if (lane == 0) {
+        hd.tmax = tmax;
+        hd.tsum = tsum;
+        hd.weight = w;
+      }
+      mbar_arrive_warp(&bars.e_full[b]);
       const float inv = some ? __fdiv_rn(1.f, tsum) : 0.f, log_tsum = some ? log2f(tsum) : 0.f;
       for (int j = lane; j < p.K; j += 32) {
         eq[j] *= inv;
         elq[j] = (elq[j] - tmax) * c - log_tsum;
       }
-      __syncwarp();
       // the same id twice?  One bit per element of the slice tells, and only then are the equal ids looked for
       bool twice = false;
       for (int j = lane; j < own; j += 32) {
@@ -537,162 +610,174 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           gq[j] = lead ? q : -1.f;
         }
       }
-      if (lane == 0) {
-        head[b].tmax = tmax;
-        head[b].tsum = tsum;
-        head[b].own = own;
+      // pass 2 has written the dense gradient: the loss, and the gradient at the entries over it
+      bool ok = !failed && mbar_wait_idle(&bars.e_empty[b], phase, 300);
+      if (!__all_sync(0xffffffffu, ok)) {
+        report_error(p.status, kErrCorrectionWait);
+        failed = 1;
+        break;
       }
-      mbar_arrive_warp(&bars.e_full[b]);
-    }
-  } else {
-    // ---------------------------------------------------------------- compute
-    int it = 0;
-    bool ok = true;
-    for (int row = first_row; row < p.T; row += plan.clusters, ++it) {
-      const int slot = it % plan.slots, b = it & 1;
-      // a wait that runs out is recorded and no further one is made; the barriers of the row are all kept
-      auto wait = [&](uint64_t* bar, uint32_t phase) {
-        if (ok && !mbar_wait(bar, phase)) {
-          report_error(p.status, kErrEpilogueWait);
-          failed[b] = 1;
-          ok = false;
-        }
-      };
-      const T* src = static_cast<const T*>(p.logits) + row * p.ld;
-      const Granules<T> gr(src, p.V);
-      // granules [gs, ge) of the slice are whole; the row's elements before the first and behind the last whole granule
-      // (fewer than n each) go to a thread of their own
-      const int g0 = rank * plan.per, whole = (gr.lead + p.V) / n;
-      const int gs = max(g0, gr.lead > 0 ? 1 : 0), ge = min(g0 + plan.per, whole);
-      const uint4* slice = reinterpret_cast<const uint4*>(dyn + slot * slice_bytes) - g0;
-      int edge = -1;
-      if (threadIdx.x < 8) {
-        if (rank == 0 && gr.lead > 0 && static_cast<int>(threadIdx.x) < min(n - gr.lead, p.V)) edge = threadIdx.x;
-      } else if (threadIdx.x < 16) {
-        const int at = whole * n - gr.lead + static_cast<int>(threadIdx.x) - 8;
-        if (whole >= g0 && whole < g0 + plan.per && (whole > 0 || gr.lead == 0) && at < p.V) edge = at;
-      }
-      const float x_edge = edge >= 0 ? Lane<T>::value(src + edge) : 0.f;
-      wait(&bars.full[slot], (it / plan.slots) & 1);
-      // pass 1: a thread that has seen nothing but -inf adds exp2(-inf) = 0
-      constexpr int kU = 4, kP = Pairs<T>::n;
-      const uint64_t c2 = pair(c, c);
-      float top = edge >= 0 ? x_edge * c : -INFINITY;
-      uint64_t acc[2] = {0, 0};                       // two pairs of sums
-      if (edge >= 0) acc[0] = pair(ex2(x_edge * c - (top == -INFINITY ? 0.f : top)), 0.f);
-      if (top != top) top = -INFINITY;
-      auto take = [&](const uint4* v, int count) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < count; ++u) m = fmaxf(m, Pairs<T>::top(v[u]));
-        m *= c;
-        if (m > top) {
-          const float scale = ex2(top - m);
-          acc[0] = mul2(acc[0], pair(scale, scale));
-          acc[1] = mul2(acc[1], pair(scale, scale));
-          top = m;
-        }
-        const float base = top == -INFINITY ? 0.f : top;
-        const uint64_t minus = pair(-base, -base);
-#pragma unroll
-        for (int u = 0; u < count; ++u) {
-          uint64_t f[kP];
-          Pairs<T>::widen(v[u], f);
-#pragma unroll
-          for (int j = 0; j < kP; ++j) acc[j & 1] = add2(acc[j & 1], ex2_2(fma2(f[j], c2, minus)));
-        }
-      };
-      int g = gs + static_cast<int>(threadIdx.x);
-      for (; g + (kU - 1) * kRowCompute < ge; g += kU * kRowCompute) {
-        uint4 v[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) v[u] = slice[g + u * kRowCompute];
-        take(v, kU);
-      }
-      for (; g < ge; g += kRowCompute) {
-        const uint4 v = slice[g];
-        take(&v, 1);
-      }
-      float sum, sum1;
-      unpair(add2(acc[0], acc[1]), sum, sum1);
-      sum += sum1;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        merge(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
-      if (lane == 0) red[b][warp] = make_float2(top, sum);
-      if (p.grad == nullptr) mbar_arrive_warp(&bars.empty[slot]);
-      compute_barrier();
-      top = red[b][lane & 7].x;
-      sum = red[b][lane & 7].y;
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1)
-        merge(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
-      // the logits at the entries have been read: only now may another CTA overwrite them
-      wait(&bars.e_full[b], (it >> 1) & 1);
-      if constexpr (C > 1) {
-        if (warp == 0) {
-          if (lane == 0) mbar_arrive_expect_tx(&bars.xchg[b], C * 8);
-          __syncwarp();
-          if (lane < C) send_pair(&part[b][rank], &bars.xchg[b], lane, top, sum);
-        }
-        wait(&bars.xchg[b], (it >> 1) & 1);
-        top = part[b][lane & (C - 1)].x;
-        sum = part[b][lane & (C - 1)].y;
-#pragma unroll
-        for (int o = C / 2; o > 0; o >>= 1)
-          merge(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
-      }
-      const float* eq = reinterpret_cast<const float*>(entry_base + b * entry_bytes(plan.kpad));
-      if (rank == 0 && warp == kRowCompute / 32 - 1) {
+      const float top = hd.top, sum = hd.sum;
+      if (rank == 0) {
         if (p.loss != nullptr) {
-          const float log_sum = log2f(sum), *elq = eq + plan.kpad, *es = elq + plan.kpad;
+          const float log_sum = log2f(sum);
           float l = 0.f;
           for (int j = lane; j < p.K; j += 32)
             l += eq[j] == 0.f ? 0.f : eq[j] * (elq[j] - (fmaf(es[j], c, -top) - log_sum));
           l = warp_total(l) * kLn2;
           if (lane == 0) p.loss[row] = l;
         }
-        if (p.stats != nullptr && lane == 0) p.stats[row] = make_float4(top, sum, head[b].tmax, head[b].tsum);
+        if (p.stats != nullptr && lane == 0) p.stats[row] = make_float4(top, sum, tmax, tsum);
+      }
+      if (p.grad != nullptr && w != 0.f) {
+        TO* dst = static_cast<TO*>(p.grad) + row * p.ldg;
+        const float rs = __fdiv_rn(1.f, sum), gw = w * p.inv_tau;
+        for (int j = lane; j < own; j += 32)
+          if (!(gq[j] < 0.f)) Lane<TO>::store(dst + oid[j], (ex2(fmaf(os[j], c, -top)) * rs - gq[j]) * gw);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---------------------------------------------------------------- compute
+    constexpr int kP = Pairs<T>::n;
+    constexpr uint32_t kNone = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;    // -inf
+    const uint64_t c2 = pair(c, c);
+    int it = 0, slot1 = 0, slot2 = 0;      // ring positions of the two passes
+    uint32_t lap = 0;
+    for (long long row = first_row; row < p.T; row += plan.clusters, ++it) {
+      const int b = it & 1;
+      const uint32_t phase = (it >> 1) & 1;
+      const T* src = static_cast<const T*>(p.logits) + row * p.ld;
+      const Granules<T> gr(src, p.V);
+      const Slice<T> sl(gr, rank, plan.per, p.V);
+      const int edge = sl.edge(gr, rank, plan.per, p.V, threadIdx.x);
+      const float x_edge = edge >= 0 ? Lane<T>::value(src + edge) : -INFINITY;
+      bool ok = true;
+      // pass 1: a thread that has seen nothing but -inf adds exp2(-inf) = 0
+      float top = -INFINITY;
+      uint64_t acc[2] = {0, 0};                       // two pairs of sums
+      auto raise = [&](float m) {
+        if (m > top) {
+          const float scale = ex2(top - m);
+          acc[0] = mul2(acc[0], pair(scale, scale));
+          acc[1] = mul2(acc[1], pair(scale, scale));
+          top = m;
+        }
+        return top == -INFINITY ? 0.f : -top;
+      };
+      auto take = [&](const uint4 (&v)[kU]) {
+        const float base = raise(Pairs<T>::top(v) * c);
+        const uint64_t minus = pair(base, base);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          uint64_t f[kP];
+          Pairs<T>::widen(v[u], f);
+#pragma unroll
+          for (int j = 0; j < kP; ++j) acc[j & 1] = add2(acc[j & 1], ex2_2(fma2(f[j], c2, minus)));
+        }
+      };
+      for (int k = 0; k < plan.chunks; ++k) {
+        const int k0 = sl.g0 + k * kChunk;
+        ok = __all_sync(0xffffffffu, mbar_wait_soon(&bars.full[slot1], lap));
+        if (!ok) break;
+        const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot1 * kChunk;
+        const int lo = sl.gs - k0, hi = min(sl.ge - k0, kChunk);
+        const int g = threadIdx.x;
+        uint4 v[kU];
+        if (lo <= 0 && hi == kChunk) {
+#pragma unroll
+          for (int u = 0; u < kU; ++u) v[u] = chunk[g + u * kRowCompute];
+          take(v);
+        } else if (g < hi) {
+#pragma unroll
+          for (int u = 0; u < kU; ++u) {
+            const int i = g + u * kRowCompute;
+            v[u] = i >= lo && i < hi ? chunk[i] : make_uint4(kNone, kNone, kNone, kNone);
+          }
+          take(v);
+        }
+        if (p.grad == nullptr) mbar_arrive_warp(&bars.empty[slot1]);
+        if (++slot1 == plan.ring) { slot1 = 0; lap ^= 1; }
+      }
+      if (edge >= 0) {
+        const float base = raise(x_edge * c);
+        acc[0] = add2(acc[0], pair(ex2(fmaf(x_edge, c, base)), 0.f));
+      }
+      float sum, sum1;
+      unpair(add2(acc[0], acc[1]), sum, sum1);
+      sum += sum1;
+      warp_merge(top, sum);
+      // the logits at the entries have been read: only now may another CTA overwrite them
+      ok = ok && mbar_wait_soon(&bars.e_full[b], phase);
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(&bars.xchg[b], C * kRowWarps * 8);
+      __syncwarp();
+      if (lane < C) send_pair(&part[b][rank * kRowWarps + warp], &bars.xchg[b], lane, top, sum);
+      ok = ok && mbar_wait_soon(&bars.xchg[b], phase);
+      if (!__all_sync(0xffffffffu, ok)) {
+        report_error(p.status, kErrEpilogueWait);
+        failed = 1;
+        break;
+      }
+      constexpr int kPairs = C * kRowWarps;
+      top = lane < kPairs ? part[b][lane].x : -INFINITY;
+      sum = lane < kPairs ? part[b][lane].y : 0.f;
+#pragma unroll
+      for (int i = 32; i < kPairs; i += 32) merge(top, sum, part[b][lane + i].x, part[b][lane + i].y);
+      warp_merge(top, sum);
+      if (threadIdx.x == 0) {
+        head[b].top = top;
+        head[b].sum = sum;
       }
       if (p.grad != nullptr) {
         TO* dst = static_cast<TO*>(p.grad) + row * p.ldg;
         const bool aligned = granules_aligned<TO, n>(dst, gr.lead);
-        const float w = p.weight != nullptr ? p.weight[row] : 1.f;
+        const float w = head[b].weight;
         // no entries, or a token that does not count: zero whatever the logits hold
         const bool zero = head[b].tsum == 0.f || w == 0.f;
-        const float inv = __fdiv_rn(1.f, sum), gw = w * p.inv_tau, scale = gw * inv;
+        const float scale = w * p.inv_tau * __fdiv_rn(1.f, sum);
         const uint64_t scale2 = pair(scale, scale), minus = pair(-top, -top);
-        TO* at = dst - gr.lead;
-#pragma unroll kU
-        for (int k = gs + static_cast<int>(threadIdx.x); k < ge; k += kRowCompute) {
+        TO* out = dst - gr.lead;
+        if (zero) {
+          const uint64_t none[kP] = {};
+          for (int g = sl.gs + static_cast<int>(threadIdx.x); g < sl.ge; g += kRowCompute)
+            store_pairs<TO, kP>(out + g * n, aligned, none);
+        }
+        auto give = [&](const uint4& v, int granule) {
           uint64_t f[kP];
-          Pairs<T>::widen(slice[k], f);
+          Pairs<T>::widen(v, f);
 #pragma unroll
           for (int j = 0; j < kP; ++j) f[j] = mul2(ex2_2(fma2(f[j], c2, minus)), scale2);
+          store_pairs<TO, kP>(out + granule * n, aligned, f);
+        };
+        for (int k = 0; k < plan.chunks; ++k) {
+          const int k0 = sl.g0 + k * kChunk;
+          const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot2 * kChunk;
+          const int lo = sl.gs - k0, hi = min(sl.ge - k0, kChunk);
+          const int g = threadIdx.x;
           if (zero) {
+          } else if (lo <= 0 && hi == kChunk) {
+            uint4 v[kU];
 #pragma unroll
-            for (int j = 0; j < kP; ++j) f[j] = 0;
+            for (int u = 0; u < kU; ++u) v[u] = chunk[g + u * kRowCompute];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) give(v[u], k0 + g + u * kRowCompute);
+          } else {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+              const int i = g + u * kRowCompute;
+              if (i >= lo && i < hi) give(chunk[i], k0 + i);
+            }
           }
-          store_pairs<TO, kP>(at + k * n, aligned, f);
+          mbar_arrive_warp(&bars.empty[slot2]);
+          if (++slot2 == plan.ring) slot2 = 0;
         }
         if (edge >= 0) Lane<TO>::store(dst + edge, zero ? 0.f : ex2(fmaf(x_edge, c, -top)) * scale);
-        mbar_arrive_warp(&bars.empty[slot]);
-        compute_barrier();                 // the dense gradient is written
-        if (!zero) {
-          const float *os = eq + 4 * plan.kpad, *gq = os + plan.kpad;
-          const int* oid = reinterpret_cast<const int*>(gq + plan.kpad);
-          for (int j = threadIdx.x; j < head[b].own; j += kRowCompute)
-            if (!(gq[j] < 0.f)) Lane<TO>::store(dst + oid[j], (ex2(fmaf(os[j], c, -top)) * inv - gq[j]) * gw);
-        }
-      } else {
-        compute_barrier();
       }
       mbar_arrive_warp(&bars.e_empty[b]);
-      if (failed[b]) break;                // set before the barrier above, so the same for all compute threads
     }
   }
   __syncthreads();
-  if (failed[0] || failed[1]) drain_delay();
+  if (failed) drain_delay();
   if constexpr (C > 1) {                   // nobody sends to a CTA that has left
     cluster_arrive();
     cluster_wait();
@@ -828,20 +913,24 @@ distill_grad_kernel(const DistillParams p, int chunks) {
 static long long max_granules(int V, int n) { return (static_cast<long long>(V) + 2 * (n - 1)) / n; }
 
 constexpr int kRowSmem = 224 * 1024;               // dynamic shared memory of an SM that the row kernel counts on
-constexpr int kRowSlice = 144 * 1024;              // largest slice: 1024 entries, the bitmap and the barriers fit beside it
+constexpr int kRowSlice = 144 * 1024;              // largest slice: 1024 entries, bitmaps and barriers fit beside it
 
 template <typename T, typename TO, int C>
 static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   constexpr int n = Lane<T>::n;
   RowPlan plan{};
   plan.per = static_cast<int>((max_granules(p.V, n) + C - 1) / C);
+  plan.chunks = (plan.per + kChunk - 1) / kChunk;
   plan.kpad = (p.K + 3) & ~3;
-  const int side = 2 * entry_bytes(plan.kpad) + bitmap_bytes(plan.per, n), slice = plan.per * 16;
-  // two CTAs per SM where two slices of each fit, so that one computes while the other waits; else one CTA
-  const int half = kRowSmem / 2 - 2048 - side, whole = kRowSmem - 2048 - side;
-  plan.slots = 2 * slice <= half ? half / slice : whole / slice;
-  plan.slots = plan.slots < 1 ? 1 : plan.slots > 4 ? 4 : plan.slots;
-  const int smem = plan.slots * slice + side;
+  const int side = 2 * (entry_bytes(plan.kpad) + bitmap_bytes(plan.per, n));
+  // two CTAs per SM where a slice fits into half of it, so that one computes while the other waits; else one CTA
+  for (int ctas = 2; ctas >= 1; --ctas) {
+    plan.ring = (kRowSmem / ctas - 2048 - side) / (kChunk * 16);
+    if (plan.ring >= plan.chunks) break;
+  }
+  if (plan.ring > kMaxChunks) plan.ring = kMaxChunks;
+  if (plan.ring < plan.chunks) return cudaErrorInvalidValue;
+  const int smem = plan.ring * kChunk * 16 + side;
   auto kernel = distill_row_kernel<T, TO, C>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -882,19 +971,18 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p, plan);
 }
 
-// CTAs per row: the fewest whose slices fit twice into half an SM's shared memory, more (up to 8) while the rows alone
-// do not fill the SMs.
-static int row_cluster(int T, int V, int n) {
-  const long long bytes = max_granules(V, n) * 16;
-  int c = 1;
-  while (c < 8 && bytes > static_cast<long long>(c) * 48 * 1024) c *= 2;
-  while (c < 8 && static_cast<long long>(T) * c < sm_count() && bytes > static_cast<long long>(c) * 4096) c *= 2;
-  return c;
-}
+// CTAs per row: the fewest whose slice of it leaves room for two CTAs on an SM, more (up to 8) while the rows alone do not
+// fill the SMs.  Measured for 4096 rows of 151936 bf16: 4 CTAs 500 us, 8 CTAs (half the slice, the same cost per row of
+// merging and exchanging) 687 us.
+constexpr int kHalfSlice = 88 * 1024;
 
 template <typename T, typename TO>
 static cudaError_t run_row(const DistillParams& p, cudaStream_t stream) {
-  switch (row_cluster(p.T, p.V, Lane<T>::n)) {
+  const long long bytes = max_granules(p.V, Lane<T>::n) * 16;
+  int c = 1;
+  while (c < 8 && bytes > static_cast<long long>(c) * kHalfSlice) c *= 2;
+  while (c < 8 && static_cast<long long>(p.T) * c < sm_count() && bytes > static_cast<long long>(c) * 4096) c *= 2;
+  switch (c) {
     case 1: return launch_row<T, TO, 1>(p, stream);
     case 2: return launch_row<T, TO, 2>(p, stream);
     case 4: return launch_row<T, TO, 4>(p, stream);
