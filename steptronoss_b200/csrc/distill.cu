@@ -908,6 +908,42 @@ distill_grad_kernel(const DistillParams p, int chunks) {
   write_entries<TO>(p, e, dst, st, w, [](int) { return true; });
 }
 
+// ------------------------------------------------------------------------------------------- fused head: total, scaling
+// sum_t w_t loss_t in a fixed order, tokens of weight 0 left out whatever their loss; one CTA, a few microseconds for the
+// tokens of a step.
+__global__ void __launch_bounds__(1024)
+distill_total_kernel(const float* __restrict__ loss, const float* __restrict__ w, int T, float* __restrict__ total) {
+  __shared__ float red[32];
+  float s = 0.f;
+  for (int t = threadIdx.x; t < T; t += 1024) s += w[t] == 0.f ? 0.f : w[t] * loss[t];
+  s = warp_total(s);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_total(red[threadIdx.x]);
+    if (threadIdx.x == 0) *total = s;
+  }
+}
+
+// bf16(x * *scale): the gradients that the forward pass left, times the incoming one.  6 bytes per element, DRAM bound.
+__global__ void __launch_bounds__(256)
+distill_scale_kernel(const float4* __restrict__ x, const float* __restrict__ scale, uint2* __restrict__ y, long long n4) {
+  const float s = *scale;
+  const long long step = static_cast<long long>(gridDim.x) * 256;
+  long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  for (; i + 3 * step < n4; i += 4 * step) {
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = __ldcs(x + i + u * step);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y[i + u * step] = make_uint2(pack_bf16(v[u].x * s, v[u].y * s), pack_bf16(v[u].z * s, v[u].w * s));
+  }
+  for (; i < n4; i += step) {
+    const float4 v = x[i];
+    y[i] = make_uint2(pack_bf16(v.x * s, v.y * s), pack_bf16(v.z * s, v.w * s));
+  }
+}
+
 // ------------------------------------------------------------------------------------------- launchers
 // Granules of a row whose start may lie anywhere in its first granule.
 static long long max_granules(int V, int n) { return (static_cast<long long>(V) + 2 * (n - 1)) / n; }
@@ -1077,5 +1113,20 @@ extern "C" int stb_distill_grad(const void* logits, long long ld, void* grad, lo
   if (elem_bytes == 2) distill_grad_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kDsThreads, 0, stream>>>(p, ch);
   else if (grad_bytes == 4) distill_grad_kernel<float, float><<<grid, kDsThreads, 0, stream>>>(p, ch);
   else distill_grad_kernel<float, __nv_bfloat16><<<grid, kDsThreads, 0, stream>>>(p, ch);
+  return -static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int stb_distill_total(const float* loss, const float* weight, int T, float* total, cudaStream_t stream) {
+  distill_total_kernel<<<1, 1024, 0, stream>>>(loss, weight, T, total);
+  return -static_cast<int>(cudaGetLastError());
+}
+
+// y (bf16) = x (fp32) * *scale; count a multiple of 4, both 16-byte aligned.
+extern "C" int stb_distill_scale(const float* x, const float* scale, void* y, long long count, cudaStream_t stream) {
+  if (count == 0) return 0;
+  if (count % 4 || (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(y) & 15)) return -kErrBadArgument;
+  const long long blocks = (count / 4 + 1023) / 1024, most = static_cast<long long>(sm_count()) * 8;
+  distill_scale_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(
+      reinterpret_cast<const float4*>(x), scale, static_cast<uint2*>(y), count / 4);
   return -static_cast<int>(cudaGetLastError());
 }

@@ -23,7 +23,6 @@ import math
 
 import torch
 import torch.distributed as dist
-from torch.autograd.function import once_differentiable
 
 from . import native
 from .cross_entropy import _all_reduce
@@ -35,6 +34,8 @@ native.register_signature("stb_distill_row_limit", [I])
 native.register_signature("stb_distill_row", [P, L, P, L, P, I, L, P, L, P, P, P, I, I, I, F, I, I, P, P])
 native.register_signature("stb_distill_stats", [P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, P])
 native.register_signature("stb_distill_loss", [P, I, L, P, L, P, P, P, I, I, L, F, P])
+native.register_signature("stb_distill_total", [P, P, I, P, P])
+native.register_signature("stb_distill_scale", [P, P, P, L, P])
 native.register_signature("stb_distill_grad", [P, L, P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, I, P])
 
 
@@ -135,10 +136,11 @@ def _fits_row(V: int, elem: int) -> bool:
     return V <= limit
 
 
-def _row_kernel(x, ids, t, temperature, weights=None, grad=None, stats=None):
+def _row_kernel(x, ids, t, temperature, weights=None, grad=None, stats=None, loss=None):
     """One pass over whole rows: the loss, and on request the gradient and the statistics."""
     T, V = x.shape
-    loss = x.new_empty(T, dtype=torch.float32)
+    if loss is None:
+        loss = x.new_empty(T, dtype=torch.float32)
     size = x.element_size()
     gp, gld, gsize = (None, 0, size) if grad is None else (grad.data_ptr(), grad.stride(0), grad.element_size())
     rc = native.launch(
@@ -152,7 +154,7 @@ def _row_kernel(x, ids, t, temperature, weights=None, grad=None, stats=None):
     return loss
 
 
-def _stats_kernels(x, ids, t, temperature, vocab_start=0, group=None):
+def _stats_kernels(x, ids, t, temperature, vocab_start=0, group=None, loss=None):
     """``(loss, statistics)`` of rows of any length, or of the shards of a group."""
     T, V = x.shape
     K, vocab, index = ids.shape[1], V * _group_size(group), x.get_device()
@@ -166,7 +168,8 @@ def _stats_kernels(x, ids, t, temperature, vocab_start=0, group=None):
     count_launch()
     if _group_size(group) > 1:
         _join_shards(stats, picked, group)
-    loss = x.new_empty(T, dtype=torch.float32)
+    if loss is None:
+        loss = x.new_empty(T, dtype=torch.float32)
     native.check(native.launch(
         lib.stb_distill_loss, index, ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0),
         stats.data_ptr(), picked.data_ptr(), loss.data_ptr(), T, K, vocab, 1.0 / temperature), "distill_loss")
@@ -202,15 +205,20 @@ def _whole_rows(x, vocab_start: int, group) -> bool:
     return vocab_start == 0 and (group is None or _group_size(group) == 1) and _fits_row(x.shape[1], x.element_size())
 
 
-def _loss_and_grad(x, ids, t, temperature, weights, grad, vocab_start=0, group=None):
+def _loss_and_grad(x, ids, t, temperature, weights, grad, vocab_start=0, group=None, loss=None):
     """Loss of the rows of ``x``, their weighted gradient into ``grad`` (which may be ``x``)."""
     if x.shape[0] == 0:
         return torch.empty(0, dtype=torch.float32, device=x.device)
     if _whole_rows(x, vocab_start, group):
-        return _row_kernel(x, ids, t, temperature, weights, grad)
-    loss, stats = _stats_kernels(x, ids, t, temperature, vocab_start, group)
+        return _row_kernel(x, ids, t, temperature, weights, grad, loss=loss)
+    loss, stats = _stats_kernels(x, ids, t, temperature, vocab_start, group, loss)
     _grad_kernel(x, ids, t, temperature, weights, stats, grad, vocab_start, x.shape[1] * _group_size(group))
     return loss
+
+
+def _first_order(what: str) -> None:
+    if torch.is_grad_enabled():              # create_graph=True
+        raise RuntimeError(f"{what} has no second derivative")
 
 
 # --------------------------------------------------------------------------------------------------- logits
@@ -236,18 +244,20 @@ class _TopkDistillationFn(torch.autograd.Function):
         return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gloss):
+        _first_order("topk_distillation")
         temperature, vocab_start, group = ctx.args
-        w = gloss.reshape(-1).float().contiguous()
+        w = gloss if gloss.dim() == 1 else gloss.reshape(-1)
+        if w.dtype != torch.float32 or not w.is_contiguous():
+            w = w.float().contiguous()
         if len(ctx.saved_tensors) == 1:
             (unit,) = ctx.saved_tensors
             return _weighted(unit, w).to(ctx.dtype).view(ctx.shape), None, None, None, None, None
         x, ids, t, stats = ctx.saved_tensors
-        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        grad = x.new_empty(x.shape)
         if x.shape[0]:
             _grad_kernel(x, ids, t, temperature, w, stats, grad, vocab_start, x.shape[1] * _group_size(group))
-        return grad.view(ctx.shape), None, None, None, None, None
+        return grad if len(ctx.shape) == 2 else grad.view(ctx.shape), None, None, None, None, None
 
 
 def topk_distillation(logits, teacher_ids, teacher_logits, temperature: float = 1.0, vocab_start: int = 0, group=None):
@@ -321,57 +331,72 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
     def forward(ctx, h, w, ids, t, weights, temperature, vocab_start, group, chunk):
         T, H = h.shape
         V = w.shape[0]
-        dev = h.device
         need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         main_grad = getattr(w, "main_grad", None) if need_dw else None
-        loss = torch.empty(T, dtype=torch.float32, device=dev)
-        dh = torch.empty((T, H), dtype=torch.float32, device=dev) if need_dh else None
+        f32 = torch.float32
+        loss, total = h.new_empty(T, dtype=f32), h.new_empty((), dtype=f32)
+        dh = h.new_empty((T, H), dtype=f32) if need_dh else None
         dw = main_grad
         if need_dw and dw is None:
-            dw = torch.empty((V, H), dtype=torch.float32, device=dev) if T else torch.zeros(
-                (V, H), dtype=torch.float32, device=dev)
+            dw = h.new_empty((V, H), dtype=f32) if T else h.new_zeros((V, H), dtype=f32)
         rows = min(chunk, T)
-        logits = torch.empty((rows, V), dtype=torch.float32, device=dev)
-        grad = torch.empty((rows, V), dtype=torch.bfloat16, device=dev) if need_dh or need_dw else None
+        logits = h.new_empty((rows, V), dtype=f32)
+        grad = h.new_empty((rows, V)) if need_dh or need_dw else None
         for t0 in range(0, T, chunk):
             n = min(T - t0, chunk)
-            s, hc = logits[:n], h[t0:t0 + n]
+            whole = n == T
+            s, hc = (logits, h) if whole else (logits[:n], h[t0:t0 + n])
             gemm(hc, w, out=s)
-            args = (s, ids[t0:t0 + n], t[t0:t0 + n], temperature)
+            args = (s, ids, t, temperature) if whole else (s, ids[t0:t0 + n], t[t0:t0 + n], temperature)
+            lc = loss if whole else loss[t0:t0 + n]
             if grad is None:
                 if _whole_rows(s, vocab_start, group):
-                    loss[t0:t0 + n] = _row_kernel(*args)
+                    _row_kernel(*args, loss=lc)
                 else:
-                    loss[t0:t0 + n] = _stats_kernels(*args, vocab_start, group)[0]
+                    _stats_kernels(*args, vocab_start, group, loss=lc)
                 continue
-            g = grad[:n]
-            loss[t0:t0 + n] = _loss_and_grad(*args, weights[t0:t0 + n], g, vocab_start, group)
+            g = grad if n == rows else grad[:n]
+            _loss_and_grad(*args, weights if whole else weights[t0:t0 + n], g, vocab_start, group, loss=lc)
             if need_dh:
-                gemm(g, w, b_mn_major=True, out=dh[t0:t0 + n])
+                gemm(g, w, b_mn_major=True, out=dh if whole else dh[t0:t0 + n])
             if need_dw:
                 gemm(g, hc, a_mn_major=True, b_mn_major=True, out=dw, accumulate=main_grad is not None or t0 > 0)
+        native.check(native.launch(native.load().stb_distill_total, h.get_device(), loss.data_ptr(), weights.data_ptr(), T,
+                                   total.data_ptr()), "distill_total")
+        count_launch()
         ctx.save_for_backward(dh)
         ctx.dw = None if main_grad is not None else dw
         ctx.w_ref = w
         ctx.used_main_grad = main_grad is not None
         ctx.mark_non_differentiable(loss)
-        return torch.where(weights == 0, 0.0, loss * weights).sum(), loss
+        return total, loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gloss, _):
+        _first_order("fused_linear_topk_distillation")
         (dh,) = ctx.saved_tensors
         gh = gw = None
+        if gloss.dtype != torch.float32:
+            gloss = gloss.float()
         if ctx.needs_input_grad[0]:
-            gh = torch.mul(dh, gloss, out=torch.empty(dh.shape, dtype=torch.bfloat16, device=dh.device))
+            gh = _scaled(dh, gloss)
         if ctx.needs_input_grad[1]:
             if ctx.used_main_grad:
                 # dW already sits in main_grad with unit upstream gradient: the loss returned by this function has to
                 # be the quantity that backward() is called on.
                 ctx.w_ref.grad_added_to_main_grad = True
             else:
-                gw = torch.mul(ctx.dw, gloss, out=torch.empty(ctx.dw.shape, dtype=torch.bfloat16, device=ctx.dw.device))
+                gw = _scaled(ctx.dw, gloss)
         return gh, gw, None, None, None, None, None, None, None
+
+
+def _scaled(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """bf16 ``x * scale`` for a contiguous fp32 matrix and a scalar on the device."""
+    y = x.new_empty(x.shape, dtype=torch.bfloat16)
+    native.check(native.launch(native.load().stb_distill_scale, x.get_device(), x.data_ptr(), scale.data_ptr(), y.data_ptr(),
+                               x.numel()), "distill_scale")
+    count_launch()
+    return y
 
 
 def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, temperature: float = 1.0,
