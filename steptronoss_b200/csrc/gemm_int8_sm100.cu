@@ -249,9 +249,11 @@ template <int BM>
 struct Int8SplitSmem {
   static constexpr int kXTile = BM * kI8BlockK;
   static constexpr int kStageBytes = kI8WTile + kXTile;
+  // two CTAs per SM (about 110 KB each)
+  static constexpr int kStages = BM == 16 ? 6 : BM == 32 ? 5 : BM == 64 ? 4 : 3;
   static constexpr int kPartBytes = kI8BlockN * BM * 4;       // [source CTA][column of this CTA][128 channels] int32
-  static constexpr int kStages = BM <= 32 ? 5 : BM == 64 ? 4 : 4;
-  static constexpr int kTotal = kStages * kStageBytes + kPartBytes + 256 + 1024;
+  static constexpr int kTotal = kStages * kStageBytes + 256 + 1024;
+  static_assert(kPartBytes <= kStages * kStageBytes, "the partial sums reuse the operand ring");
 };
 
 __device__ __forceinline__ uint32_t i8_cluster_rank() {
@@ -259,12 +261,20 @@ __device__ __forceinline__ uint32_t i8_cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void i8_cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // One output tile (128 channels, BM tokens) per cluster of S CTAs; CTA r takes every k block kb with kb % S == r.
-// After the products, column c of the tile belongs to CTA c % S: every CTA stores its partial sums of that column into
-// that CTA's shared memory, and after one cluster barrier each CTA adds, scales and writes its columns.
+// When all products of the cluster are done, column c of the tile belongs to CTA c % S: every CTA stores its partial sums
+// of that column into that CTA's shared memory (over the operand ring, which nobody reads any more), and after one more
+// cluster barrier each CTA adds, scales and writes its columns.
+//
+// Bound: the weights' bytes.  Two CTAs fit on an SM, so up to 296 stream at a time and none waits for a second wave.
 template <int BM, int S, typename TY>
-__global__ void __launch_bounds__(kI8Threads)
+__global__ void __launch_bounds__(kI8Threads, 2)
 gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                        const Int8GemmParams p) {
   using L = Int8SplitSmem<BM>;
@@ -273,8 +283,8 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   extern __shared__ uint8_t smem_raw[];
   // the same offset in every CTA of the cluster: the dynamic segment starts at the same address in all of them
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int* part = reinterpret_cast<int*>(smem + kStages * L::kStageBytes);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kStages * L::kStageBytes + L::kPartBytes);
+  int* part = reinterpret_cast<int*>(smem);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kStages * L::kStageBytes);
   uint64_t* empty_bar = full_bar + kStages;
   uint64_t* done_bar = empty_bar + kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
@@ -289,6 +299,13 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   const int all_blocks = (p.K + kI8BlockK - 1) / kI8BlockK;
   const int k_blocks = (all_blocks - rank + S - 1) / S;     // one at least: S is at most half of all_blocks
 
+  auto load = [&](int i) {
+    const int s = i % kStages, kb = i * S + rank;
+    uint8_t* sw = smem + s * L::kStageBytes;
+    mbar_arrive_expect_tx(&full_bar[s], L::kStageBytes);
+    tma_load_2d(sw, &tmap_w, &full_bar[s], kb * kI8BlockK, n_tile * kI8BlockN);
+    tma_load_2d(sw + kI8WTile, &tmap_x, &full_bar[s], kb * kI8BlockK, m0);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -297,8 +314,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&tmap_w);
-    tma_prefetch_desc(&tmap_x);
+    for (int i = 0; i < min(kStages, k_blocks); ++i) load(i);     // on their way while the rest is set up
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, kTmemCols);
@@ -307,23 +323,17 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if constexpr (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // running
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < k_blocks; ++i) {
-        const int s = i % kStages;
-        if (!mbar_wait(&empty_bar[s], ((i / kStages) & 1) ^ 1)) {
+      for (int i = kStages; i < k_blocks; ++i) {
+        if (!mbar_wait(&empty_bar[i % kStages], ((i / kStages) & 1) ^ 1)) {
           report_error(p.status, kErrProducerWait);
           *abort_flag = 1;
           break;
         }
-        const int kb = i * S + rank;
-        uint8_t* sw = smem + s * L::kStageBytes;
-        mbar_arrive_expect_tx(&full_bar[s], L::kStageBytes);
-        tma_load_2d(sw, &tmap_w, &full_bar[s], kb * kI8BlockK, n_tile * kI8BlockN);
-        tma_load_2d(sw + kI8WTile, &tmap_x, &full_bar[s], kb * kI8BlockK, m0);
+        load(i);
       }
     }
     __syncwarp();
@@ -346,20 +356,14 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   }
   const int quarter = warp & 3;
   const int row = quarter * 32 + lane;
-  bool ok = true;
-  if (warp >= 2) {
-    ok = mbar_wait(done_bar, 0);
-    ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
-    if (!ok) report_error(p.status, kErrEpilogueWait);
-    tc_fence_after();
-  }
-  if constexpr (S > 1) {
-    __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
-  // columns of the tile in groups of 16; with S > 1 each goes to the CTA that owns it
   const int n = n_tile * kI8BlockN + row;
   const float swn = warp >= 2 && n < p.N ? p.sw[n] : 0.f;
+  bool ok = mbar_wait(done_bar, 0);           // every warp: the cluster barrier below says that this CTA's products are done
+  ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
+  if (!ok) { report_error(p.status, kErrEpilogueWait); *abort_flag = 1; }
+  tc_fence_after();
+  if constexpr (S > 1) i8_cluster_sync();
+  // columns of the tile in groups of 16; with S > 1 each goes to the CTA that owns it
   if (warp >= 2 && ok) {
     for (int c = 0; c < cols; c += 16) {
       uint32_t v[16];
@@ -382,9 +386,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     }
   }
   if constexpr (S > 1) {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    i8_cluster_sync();
     if (warp >= 2 && n < p.N) {
       for (int slot = 0; slot * S + rank < cols; ++slot) {
         int sum = 0;
@@ -475,8 +477,8 @@ template <int BM, typename TY>
 static int run_split(const void* xq, const void* wq, const Int8GemmParams& p, long long ldx, long long ldw, cudaStream_t stream) {
   const long long tiles = static_cast<long long>((p.N + kI8BlockN - 1) / kI8BlockN) * ((p.M + BM - 1) / BM);
   const int blocks = (p.K + kI8BlockK - 1) / kI8BlockK;
-  int s = 1;   // enough CTAs for every SM, each with two k blocks at least
-  while (s < 8 && tiles * s < sm_count() && blocks >= 4 * s) s *= 2;
+  int s = 1;   // as many CTAs as the SMs hold two of, each with two k blocks at least
+  while (s < 8 && tiles * s * 2 <= 2 * sm_count() && blocks >= 4 * s) s *= 2;
   switch (s) {
     case 1: return launch_split<BM, 1, TY>(xq, wq, p, ldx, ldw, tiles, stream);
     case 2: return launch_split<BM, 2, TY>(xq, wq, p, ldx, ldw, tiles, stream);
