@@ -9,7 +9,7 @@
 // columns), whatever their number: a decode step of a few tokens then takes a 16-, 32- or 64-column tile instead of
 // a mostly empty 128-row one, and a warp that reads one column writes 32 neighbouring channels of one token.
 //
-//   gemm_int8_kernel        many tokens: persistent, 128 x 256 tiles, accumulators double-buffered in TMEM
+//   gemm_int8_pair_kernel   many tokens: persistent, 256 x 256 tiles on pairs of CTAs, accumulators double-buffered in TMEM
 //   gemm_int8_split_kernel  few tokens: one tile per cluster, K cut over the CTAs of the cluster so that the weights
 //                           stream through all SMs; partial sums meet in distributed shared memory
 #include "common.cuh"
@@ -63,19 +63,94 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "memory");
 }
 
-// ------------------------------------------------------------------------------------------------- many tokens
-template <int BM>                   // tokens per tile
-struct Int8Smem {
-  static constexpr int kStages = BM == 256 ? 4 : 6;
-  static constexpr int kXTile = BM * kI8BlockK;
-  static constexpr int kStageBytes = kI8WTile + kXTile;
-  static constexpr int kStoreBytes = 4 * 2 * 4096;    // per epilogue warp: two tiles of 64 tokens x 32 channels bf16
-  static constexpr int kTotal = kStages * kStageBytes + kStoreBytes + 256 + 1024;
-};
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
-// Tiles are walked in bands of kBand channel tiles so that the CTAs of a wave share weights and tokens in L2.
+// ------------------------------------------------------------------------------------------------- many tokens
+// CTA pairs (cta_group::2): a tile of 256 channels x 256 tokens on two SMs.  CTA r of the pair loads 128 channels and 128
+// tokens, a quarter less than a 128 x 256 tile of its own would take, and the tensor cores of both read both halves of
+// the tokens; the first CTA issues the products, each holds the sums of its own 128 channels (256 TMEM columns, two
+// buffers) and writes them.  What bounds the single-CTA form is the traffic from L2 to the SMs: 48 KB per 512 cycles of
+// products, of which about 58 bytes a cycle and SM arrive (128 x 256 tiles measured 2513 TOPS, 656 us for 8192 x 24576 x
+// 4096); a pair needs 32 KB.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Address of `p` in the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+// A tile into this CTA's shared memory, counted on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* d, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(d)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+// Arrive on the barrier at this offset in both CTAs once the products issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Bounded wait for an arrival that another CTA of the cluster may have made.
+__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+    if (i == 0) t0 = global_timer_ns();
+    else if ((i & 255u) == 0 && global_timer_ns() - t0 > kWaitBudgetNs) return false;
+  }
+  return false;
+}
+// The pair's products of one k block: M = 256 (128 rows of A in each CTA), N = 256 (128 rows of B in each).
+__device__ __forceinline__ void umma4_s8_pair(uint32_t d, uint64_t a0, uint64_t b0, uint32_t idesc, uint32_t accumulate) {
+  const uint64_t a1 = umma_desc_advance(a0, 32), a2 = umma_desc_advance(a0, 64), a3 = umma_desc_advance(a0, 96);
+  const uint64_t b1 = umma_desc_advance(b0, 32), b2 = umma_desc_advance(b0, 64), b3 = umma_desc_advance(b0, 96);
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %10, 0;\n\t"
+      "setp.eq.b32 q, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %5, %9, p;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %2, %6, %9, q;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %3, %7, %9, q;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %4, %8, %9, q;\n\t}"
+      ::"r"(d), "l"(a0), "l"(a1), "l"(a2), "l"(a3), "l"(b0), "l"(b1), "l"(b2), "l"(b3), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+constexpr int kPairTile = 256;                                   // channels and tokens of a pair's tile
+constexpr int kPairStages = 6;
+constexpr int kPairStageBytes = kI8WTile + 128 * kI8BlockK;      // of one CTA
+constexpr int kPairStoreBytes = 4 * 2 * 4096;                    // per epilogue warp: two tiles of 64 tokens x 32 channels
+constexpr int kPairSmem = kPairStages * kPairStageBytes + kPairStoreBytes + 256 + 1024;
+
+// Tiles are walked in bands of kBand channel tiles so that the pairs of a wave share weights and tokens in L2.
 __device__ __forceinline__ void int8_tile(int tile, int num_n, int num_m, int& n_tile, int& m_tile) {
-  constexpr int kBand = 16;
+  constexpr int kBand = 8;
   const int band = tile / (kBand * num_m);
   const int first = band * kBand;
   const int rows = min(num_n - first, kBand);
@@ -89,93 +164,92 @@ __device__ __forceinline__ void store_y(TY* p, float v);
 template <> __device__ __forceinline__ void store_y<float>(float* p, float v) { *p = v; }
 template <> __device__ __forceinline__ void store_y<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <int BM, typename TY>
+template <typename TY>
 __global__ void __launch_bounds__(kI8Threads, 1)
-gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                 const __grid_constant__ CUtensorMap tmap_y, const Int8GemmParams p) {
-  using S = Int8Smem<BM>;
-  constexpr int kStages = S::kStages;
+gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                      const __grid_constant__ CUtensorMap tmap_y, const Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
+  // the same offset in both CTAs: the dynamic segment starts at the same address in all CTAs of a cluster
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* store_stage = smem + kStages * S::kStageBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(store_stage + S::kStoreBytes);
-  uint64_t* empty_bar = full_bar + kStages;
-  uint64_t* tmem_full = empty_bar + kStages;
-  uint64_t* tmem_empty = tmem_full + 2;
+  uint8_t* store_stage = smem + kPairStages * kPairStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(store_stage + kPairStoreBytes);   // used in the first CTA
+  uint64_t* empty_bar = full_bar + kPairStages;                                      // one in each CTA
+  uint64_t* tmem_full = empty_bar + kPairStages;                                     // one in each CTA
+  uint64_t* tmem_empty = tmem_full + 2;                                              // used in the first CTA
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_n = (p.N + kI8BlockN - 1) / kI8BlockN;
-  const int num_m = (p.M + BM - 1) / BM;
-  const int num_tiles = num_n * num_m;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int num_n = (p.N + kPairTile - 1) / kPairTile;
+  const int num_m = (p.M + kPairTile - 1) / kPairTile;
+  const int num_tiles = num_n * num_m, pairs = gridDim.x / 2;
   const int k_blocks = (p.K + kI8BlockK - 1) / kI8BlockK;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
-      mbar_init(&tmem_empty[a], 4);
+      mbar_init(&tmem_empty[a], 8);          // four epilogue warps of each CTA
     }
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_x);
   }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, 2 * BM);
-    tmem_relinquish();
-  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 2 * kPairTile);
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();                        // the other CTA's barriers are initialised, too
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
-      for (int tile = blockIdx.x; tile < num_tiles && !*abort_flag; tile += gridDim.x) {
+      for (int tile = blockIdx.x / 2; tile < num_tiles && !*abort_flag; tile += pairs) {
         int n_tile, m_tile;
         int8_tile(tile, num_n, num_m, n_tile, m_tile);
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&empty_bar[s], ((it / kStages) & 1) ^ 1)) {
+          const int s = it % kPairStages;
+          if (!mbar_wait_pair(&empty_bar[s], ((it / kPairStages) & 1) ^ 1)) {
             report_error(p.status, kErrProducerWait);
             *abort_flag = 1;
             break;
           }
-          uint8_t* sw = smem + s * S::kStageBytes;
-          mbar_arrive_expect_tx(&full_bar[s], S::kStageBytes);
-          tma_load_2d(sw, &tmap_w, &full_bar[s], kb * kI8BlockK, n_tile * kI8BlockN);
-          tma_load_2d(sw + kI8WTile, &tmap_x, &full_bar[s], kb * kI8BlockK, m_tile * BM);
+          uint8_t* sw = smem + s * kPairStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kPairStageBytes);     // both CTAs' loads
+          const uint32_t bar = peer_smem(&full_bar[s], 0);
+          tma_load_2d_pair(sw, &tmap_w, bar, kb * kI8BlockK, n_tile * kPairTile + rank * 128);
+          tma_load_2d_pair(sw + kI8WTile, &tmap_x, bar, kb * kI8BlockK, m_tile * kPairTile + rank * 128);
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc_s8(kI8BlockN, BM);
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = umma_idesc_s8(256, 256);
       uint32_t it = 0, local = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok && !*abort_flag; tile += gridDim.x, ++local) {
+      for (int tile = blockIdx.x / 2; tile < num_tiles && ok && !*abort_flag; tile += pairs, ++local) {
         const int acc = local & 1;
-        ok = mbar_wait(&tmem_empty[acc], ((local >> 1) & 1) ^ 1);
+        ok = mbar_wait_pair(&tmem_empty[acc], ((local >> 1) & 1) ^ 1);
         if (!ok) { report_error(p.status, kErrMmaWaitTmem); break; }
         tc_fence_after();
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-          const int s = it % kStages;
-          ok = mbar_wait(&full_bar[s], (it / kStages) & 1);
+          const int s = it % kPairStages;
+          ok = mbar_wait_pair(&full_bar[s], (it / kPairStages) & 1);
           if (!ok) { report_error(p.status, kErrMmaWaitFull); break; }
           tc_fence_after();
-          const uint32_t sw = smem_u32(smem + s * S::kStageBytes);
-          umma4_s8(tmem_base + acc * BM, umma_smem_desc(sw, 16, 1024), umma_smem_desc(sw + kI8WTile, 16, 1024), idesc,
-                   kb > 0 ? 1u : 0u);
-          umma_commit(&empty_bar[s]);
+          const uint32_t sw = smem_u32(smem + s * kPairStageBytes);
+          umma4_s8_pair(tmem_base + acc * kPairTile, umma_smem_desc(sw, 16, 1024), umma_smem_desc(sw + kI8WTile, 16, 1024),
+                        idesc, kb > 0 ? 1u : 0u);
+          umma_commit_pair(&empty_bar[s]);
         }
         if (!ok) break;
-        umma_commit(&tmem_full[acc]);
+        umma_commit_pair(&tmem_full[acc]);
       }
       if (!ok) *abort_flag = 1;
     }
@@ -183,22 +257,22 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     const int quarter = warp & 3;
     uint8_t* my_stage = store_stage + (warp - 2) * 8192;
     uint32_t local = 0, stores = 0;
-    for (int tile = blockIdx.x; tile < num_tiles && !*abort_flag; tile += gridDim.x, ++local) {
+    for (int tile = blockIdx.x / 2; tile < num_tiles && !*abort_flag; tile += pairs, ++local) {
       int n_tile, m_tile;
       int8_tile(tile, num_n, num_m, n_tile, m_tile);
       const int acc = local & 1;
-      const int n = n_tile * kI8BlockN + quarter * 32 + lane, m0 = m_tile * BM;
+      const int n0 = n_tile * kPairTile + rank * 128 + quarter * 32, n = n0 + lane, m0 = m_tile * kPairTile;
       const float sw = n < p.N ? p.sw[n] : 0.f;
-      bool ok = mbar_wait(&tmem_full[acc], (local >> 1) & 1);
+      bool ok = mbar_wait_pair(&tmem_full[acc], (local >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) { report_error(p.status, kErrEpilogueWait); *abort_flag = 1; break; }
       tc_fence_after();
-      const int cols = min(BM, p.M - m0);
+      const int cols = min(kPairTile, p.M - m0);
 #pragma unroll 1
       for (int c = 0; c < cols; c += 32) {
         const float sx = c + lane < cols ? p.sx[m0 + c + lane] : 0.f;
         uint32_t v[32];
-        tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BM + c, v);
+        tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kPairTile + c, v);
         tmem_wait_ld();
         if (p.tma_out) {
           uint8_t* buf = my_stage + (stores & 1) * 4096;
@@ -214,7 +288,6 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              const int n0 = n_tile * kI8BlockN + quarter * 32;
               if (n0 < p.N) tma_store_2d(&tmap_y, buf, n0, m0 + (c & ~63));   // rows and channels past the end are clipped
               tma_store_commit();
             }
@@ -230,17 +303,18 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         }
       }
       tc_fence_before();
-      mbar_arrive_warp(&tmem_empty[acc]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(peer_smem(&tmem_empty[acc], 0));
     }
     if (lane == 0) tma_store_wait<0>();
   }
 
   __syncthreads();
   if (*abort_flag) drain_delay();
-  __syncthreads();
+  cluster_sync_all();                        // nobody signals or reads a CTA that has left
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 2 * BM);
+    tmem_dealloc_pair(tmem_base, 2 * kPairTile);
   }
 }
 
@@ -255,17 +329,6 @@ struct Int8SplitSmem {
   static constexpr int kTotal = kStages * kStageBytes + 256 + 1024;
   static_assert(kPartBytes <= kStages * kStageBytes, "the partial sums reuse the operand ring");
 };
-
-__device__ __forceinline__ uint32_t i8_cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void i8_cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 // One output tile (128 channels, BM tokens) per cluster of S CTAs; CTA r takes every k block kb with kb % S == r.
 // When all products of the cluster are done, column c of the tile belongs to CTA c % S: every CTA stores its partial sums
@@ -291,7 +354,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = S > 1 ? static_cast<int>(i8_cluster_rank()) : 0;
+  const int rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int num_n = (p.N + kI8BlockN - 1) / kI8BlockN;
   const int tile = blockIdx.x / S;
   const int n_tile = tile % num_n, m_tile = tile / num_n;
@@ -362,7 +425,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
   if (!ok) { report_error(p.status, kErrEpilogueWait); *abort_flag = 1; }
   tc_fence_after();
-  if constexpr (S > 1) i8_cluster_sync();
+  if constexpr (S > 1) cluster_sync_all();
   // columns of the tile in groups of 16; with S > 1 each goes to the CTA that owns it
   if (warp >= 2 && ok) {
     for (int c = 0; c < cols; c += 16) {
@@ -386,7 +449,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     }
   }
   if constexpr (S > 1) {
-    i8_cluster_sync();
+    cluster_sync_all();
     if (warp >= 2 && n < p.N) {
       for (int slot = 0; slot * S + rank < cols; ++slot) {
         int sum = 0;
@@ -427,10 +490,10 @@ static int maps_wx(CUtensorMap& tw, CUtensorMap& tx, const void* xq, const void*
   return make_tmap_2d(&tx, xq, 1, p.K, p.M, static_cast<uint64_t>(ldx), kI8BlockK, bm, 1);
 }
 
-template <int BM, typename TY>
-static int launch_int8(const void* xq, const void* wq, Int8GemmParams p, long long ldx, long long ldw, cudaStream_t stream) {
+template <typename TY>
+static int launch_pair(const void* xq, const void* wq, Int8GemmParams p, long long ldx, long long ldw, cudaStream_t stream) {
   CUtensorMap tw, tx, ty;
-  int r = maps_wx(tw, tx, xq, wq, p, ldx, ldw, BM);
+  int r = maps_wx(tw, tx, xq, wq, p, ldx, ldw, 128);
   if (r) return r;
   p.tma_out = sizeof(TY) == 2 && p.ldy % 8 == 0 && reinterpret_cast<uintptr_t>(p.Y) % 16 == 0;
   if (p.tma_out) {
@@ -440,13 +503,23 @@ static int launch_int8(const void* xq, const void* wq, Int8GemmParams p, long lo
     ty = tw;
   }
   static unsigned long long done = 0;
-  cudaError_t e = allow_smem(gemm_int8_kernel<BM, TY>, Int8Smem<BM>::kTotal, done);
+  cudaError_t e = allow_smem(gemm_int8_pair_kernel<TY>, kPairSmem, done);
   if (e != cudaSuccess) return -static_cast<int>(e);
-  const long long tiles = static_cast<long long>((p.N + kI8BlockN - 1) / kI8BlockN) * ((p.M + BM - 1) / BM);
-  if (tiles > 0x7FFFFFFFll) return -kErrBadArgument;
-  const int grid = tiles < sm_count() ? static_cast<int>(tiles) : sm_count();
-  gemm_int8_kernel<BM, TY><<<grid, kI8Threads, Int8Smem<BM>::kTotal, stream>>>(tw, tx, ty, p);
-  return -static_cast<int>(cudaGetLastError());
+  const long long tiles = static_cast<long long>((p.N + kPairTile - 1) / kPairTile) * ((p.M + kPairTile - 1) / kPairTile);
+  if (tiles > 0x3FFFFFFFll) return -kErrBadArgument;
+  const int most = sm_count() / 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < most ? tiles : most));
+  cfg.blockDim = dim3(kI8Threads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return -static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<TY>, tw, tx, ty, p));
 }
 
 template <int BM, int S, typename TY>
@@ -492,10 +565,10 @@ static int run_int8(const void* xq, const void* wq, const Int8GemmParams& p, lon
   if (p.M <= 16) return run_split<16, TY>(xq, wq, p, ldx, ldw, stream);
   if (p.M <= 32) return run_split<32, TY>(xq, wq, p, ldx, ldw, stream);
   if (p.M <= 64) return run_split<64, TY>(xq, wq, p, ldx, ldw, stream);
-  const long long n_tiles = (p.N + kI8BlockN - 1) / kI8BlockN;
-  if (n_tiles * ((p.M + 127) / 128) < sm_count()) return run_split<128, TY>(xq, wq, p, ldx, ldw, stream);
-  if (n_tiles * ((p.M + 255) / 256) < 2 * sm_count()) return launch_int8<128, TY>(xq, wq, p, ldx, ldw, stream);
-  return launch_int8<256, TY>(xq, wq, p, ldx, ldw, stream);
+  // 128 tokens fill half a pair's tile, and a product with few pair tiles leaves SMs idle: 128 x 128 tiles with K cut
+  const long long pair_tiles = static_cast<long long>((p.N + kPairTile - 1) / kPairTile) * ((p.M + kPairTile - 1) / kPairTile);
+  if (p.M <= 128 || pair_tiles * 2 < sm_count() / 2) return run_split<128, TY>(xq, wq, p, ldx, ldw, stream);
+  return launch_pair<TY>(xq, wq, p, ldx, ldw, stream);
 }
 
 }  // namespace stb
