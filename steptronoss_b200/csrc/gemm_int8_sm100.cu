@@ -126,6 +126,17 @@ __device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity) {
   }
   return false;
 }
+// Whether `ok` holds for all 128 threads that meet at named barrier `id`.
+__device__ __forceinline__ bool group_and(int id, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
+      "bar.red.and.pred q, %1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r) : "r"(id), "r"(static_cast<uint32_t>(ok)) : "memory");
+  return r != 0;
+}
 // The pair's products of one k block: M = 256 (128 rows of A in each CTA), N = 256 (128 rows of B in each).
 __device__ __forceinline__ void umma4_s8_pair(uint32_t d, uint64_t a0, uint64_t b0, uint32_t idesc, uint32_t accumulate) {
   const uint64_t a1 = umma_desc_advance(a0, 32), a2 = umma_desc_advance(a0, 64), a3 = umma_desc_advance(a0, 96);
@@ -145,7 +156,8 @@ __device__ __forceinline__ void umma4_s8_pair(uint32_t d, uint64_t a0, uint64_t 
 constexpr int kPairTile = 256;                                   // channels and tokens of a pair's tile
 constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = kI8WTile + 128 * kI8BlockK;      // of one CTA
-constexpr int kPairStoreBytes = 4 * 2 * 4096;                    // per epilogue warp: two tiles of 64 tokens x 32 channels
+constexpr int kPairStoreBytes = 2 * 2 * 32 * 128 * 2;            // two groups of epilogue warps, two chunks each
+constexpr int kPairThreads = 320;                                // producer, MMA issuer, eight epilogue warps
 constexpr int kPairSmem = kPairStages * kPairStageBytes + kPairStoreBytes + 256 + 1024;
 
 // Tiles are walked in bands of kBand channel tiles so that the pairs of a wave share weights and tokens in L2.
@@ -165,7 +177,7 @@ template <> __device__ __forceinline__ void store_y<float>(float* p, float v) { 
 template <> __device__ __forceinline__ void store_y<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 template <typename TY>
-__global__ void __launch_bounds__(kI8Threads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                       const __grid_constant__ CUtensorMap tmap_y, const Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -193,7 +205,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
-      mbar_init(&tmem_empty[a], 8);          // four epilogue warps of each CTA
+      mbar_init(&tmem_empty[a], 16);         // eight epilogue warps of each CTA
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -254,51 +266,81 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       if (!ok) *abort_flag = 1;
     }
   } else {
-    const int quarter = warp & 3;
-    uint8_t* my_stage = store_stage + (warp - 2) * 8192;
+    // eight warps: two groups of four, which take the tile's chunks of 32 tokens in turn
+    const int quarter = warp & 3, group = (warp - 2) >> 2;
+    uint8_t* my_stage = store_stage + (warp - 2) * 4096;                  // two buffers of 32 tokens x 32 channels
+    __nv_bfloat16* group_stage = reinterpret_cast<__nv_bfloat16*>(store_stage + group * 16384);   // two of 32 x 128
     uint32_t local = 0, stores = 0;
-    for (int tile = blockIdx.x / 2; tile < num_tiles && !*abort_flag; tile += pairs, ++local) {
+    for (int tile = blockIdx.x / 2; tile < num_tiles; tile += pairs, ++local) {
       int n_tile, m_tile;
       int8_tile(tile, num_n, num_m, n_tile, m_tile);
       const int acc = local & 1;
-      const int n0 = n_tile * kPairTile + rank * 128 + quarter * 32, n = n0 + lane, m0 = m_tile * kPairTile;
+      const int cta_n0 = n_tile * kPairTile + rank * 128;
+      const int n0 = cta_n0 + quarter * 32, n = n0 + lane, m0 = m_tile * kPairTile;
       const float sw = n < p.N ? p.sw[n] : 0.f;
-      bool ok = mbar_wait_pair(&tmem_full[acc], (local >> 1) & 1);
-      ok = __all_sync(0xffffffffu, ok);
+      // the group goes on or leaves as one: its warps meet at barriers below
+      const bool ok = group_and(1 + group, mbar_wait_pair(&tmem_full[acc], (local >> 1) & 1));
       if (!ok) { report_error(p.status, kErrEpilogueWait); *abort_flag = 1; break; }
       tc_fence_after();
       const int cols = min(kPairTile, p.M - m0);
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 32) {
+      for (int c = group * 32; c < cols; c += 64) {
         const float sx = c + lane < cols ? p.sx[m0 + c + lane] : 0.f;
         uint32_t v[32];
         tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kPairTile + c, v);
         tmem_wait_ld();
-        if (p.tma_out) {
-          uint8_t* buf = my_stage + (stores & 1) * 4096;
-          if ((c & 32) == 0 && stores >= 2) {
-            if (lane == 0) tma_store_wait_read<1>();
-            __syncwarp();
-          }
-          __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(buf) + (c & 32) * 32 + lane;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            out[j * 32] = __float2bfloat16_rn(static_cast<float>(static_cast<int>(v[j])) * __shfl_sync(0xffffffffu, sx, j) * sw);
-          if ((c & 32) != 0 || c + 32 >= cols) {   // 64 tokens staged, or the last of the tile
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (n0 < p.N) tma_store_2d(&tmap_y, buf, n0, m0 + (c & ~63));   // rows and channels past the end are clipped
-              tma_store_commit();
-            }
-            ++stores;
-          }
-        } else {
+        auto value = [&](int j) {
+          return static_cast<float>(static_cast<int>(v[j])) * __shfl_sync(0xffffffffu, sx, j) * sw;
+        };
+        if constexpr (sizeof(TY) == 4) {
           TY* y = static_cast<TY*>(p.Y) + static_cast<long long>(m0 + c) * p.ldy + n;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float f = static_cast<float>(static_cast<int>(v[j])) * __shfl_sync(0xffffffffu, sx, j) * sw;
+            const float f = value(j);
             if (n < p.N && c + j < cols) store_y<TY>(y + j * p.ldy, f);
+          }
+        } else if (p.tma_out) {
+          if (stores >= 2) {
+            if (lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+          }
+          uint8_t* buf = my_stage + (stores++ & 1) * 2048;
+          __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(buf) + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) out[j * 32] = __float2bfloat16_rn(value(j));
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (n0 < p.N) tma_store_2d(&tmap_y, buf, n0, m0 + c);   // rows and channels past the end are clipped
+            tma_store_commit();
+          }
+        } else {
+          // rows on any address: the group's 128 channels of a token lie side by side in shared memory and leave as
+          // 16-byte stores from the first 16-byte boundary on, what is before and behind them element by element.  (With
+          // one 2-byte store per channel 1333 x 5001 x 2050 took 42 us instead of XXX.)
+          __nv_bfloat16* buf = group_stage + (stores++ & 1) * (32 * 128);
+          __nv_bfloat16* out = buf + quarter * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) out[j * 128] = __float2bfloat16_rn(value(j));
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+          const int l = lane & 15, width = min(128, p.N - cta_n0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = quarter * 8 + i * 2 + (lane >> 4);
+            if (c + t >= cols || width <= 0) continue;
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.Y) + static_cast<long long>(m0 + c + t) * p.ldy + cta_n0;
+            const uint16_t* src = reinterpret_cast<const uint16_t*>(buf) + t * 128;
+            const int head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / 2, width);
+            const int vecs = (width - head) / 8;
+            if (l < vecs) {
+              const uint16_t* e = src + head + l * 8;
+              uint32_t u[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) u[k] = e[2 * k] | (static_cast<uint32_t>(e[2 * k + 1]) << 16);
+              *reinterpret_cast<uint4*>(dst + head + l * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+            const int at = l < 8 ? l : head + vecs * 8 + l - 8;
+            if (l < 8 ? l < head : at < width) reinterpret_cast<uint16_t*>(dst)[at] = src[at];
           }
         }
       }
@@ -451,6 +493,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   if constexpr (S > 1) {
     cluster_sync_all();
     if (warp >= 2 && n < p.N) {
+#pragma unroll 4
       for (int slot = 0; slot * S + rank < cols; ++slot) {
         int sum = 0;
 #pragma unroll
@@ -497,7 +540,7 @@ static int launch_pair(const void* xq, const void* wq, Int8GemmParams p, long lo
   if (r) return r;
   p.tma_out = sizeof(TY) == 2 && p.ldy % 8 == 0 && reinterpret_cast<uintptr_t>(p.Y) % 16 == 0;
   if (p.tma_out) {
-    r = make_tmap_2d(&ty, p.Y, 2, p.N, p.M, static_cast<uint64_t>(p.ldy) * 2, 32, 64, 0);
+    r = make_tmap_2d(&ty, p.Y, 2, p.N, p.M, static_cast<uint64_t>(p.ldy) * 2, 32, 32, 0);
     if (r) return r;
   } else {
     ty = tw;
@@ -510,7 +553,7 @@ static int launch_pair(const void* xq, const void* wq, Int8GemmParams p, long lo
   const int most = sm_count() / 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < most ? tiles : most));
-  cfg.blockDim = dim3(kI8Threads);
+  cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
