@@ -161,7 +161,7 @@ norm_quant_kernel(const NormQuantParams p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
     }
-    rstd = rsqrtf(row_sum<TPR>(ss, red_sum) / p.H + p.eps);
+    rstd = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(ss, red_sum), static_cast<float>(p.H)) + p.eps);
   }
   const float woff = p.zero_centered ? 1.f : 0.f;
 
@@ -173,7 +173,7 @@ norm_quant_kernel(const NormQuantParams p) {
     float g[8];
     widen8(k < nvec ? load8<VEC>(p.w, k * 8, p.H) : make_uint4(0, 0, 0, 0), g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= rstd * (g[j] + woff);
+    for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * (g[j] + woff);
   };
   auto top_of = [](const float (&f)[8]) {
     uint32_t m = 0;
