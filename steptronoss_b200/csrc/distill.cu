@@ -272,8 +272,10 @@ __device__ __forceinline__ void block_merge(float& m, float& s, float2* red) {
 }
 
 // ------------------------------------------------------------------------------------------- whole rows, one pass
-// Persistent clusters of C CTAs; a cluster takes every (number of clusters)-th row and each of its CTAs a contiguous
-// slice of the row's granules, which stays in shared memory between the two passes over it:
+// One cluster of C CTAs is launched per row; a running cluster takes over the rows of clusters that have not started
+// (clusterlaunchcontrol), so that its set-up is paid once and a cluster on less busy SMs does more rows (with fixed rows
+// the first clusters were done after 385 us of 495).  Each CTA has a contiguous slice of the row's granules, which stays
+// in shared memory between the two passes over it:
 //
 //   producer warp   bulk copies of 16 KB chunks into a ring that runs on from row to row: a chunk that pass 2 has read is
 //                   filled with the next row's logits at once
@@ -296,13 +298,13 @@ struct RowPlan {
   int per;             // granules per CTA
   int chunks;          // per slice
   int ring;            // chunks in shared memory, at least those of a slice
-  int clusters;
   int kpad;            // K rounded up to 4
 };
 struct RowBars {
   uint64_t full[kMaxChunks], empty[kMaxChunks];
   uint64_t e_full[2], e_empty[2];   // entries prepared; pass 2 of their row done
   uint64_t xchg[2];                 // the cluster's pairs
+  uint64_t claim[4];                // answers to the requests for further rows
 };
 // Entries of a row, arrays of kpad: for the loss q, log2 q, s; of this CTA's slice q, s, the q of the gradient (summed
 // over equal ids, -1: another entry carries it), id.
@@ -430,6 +432,31 @@ __device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t phase, un
   return false;
 }
 
+// Request for the row of a cluster that has not started; the answer goes to every CTA of this cluster.
+template <int C>
+__device__ __forceinline__ void request_row(uint4* answer, uint64_t* bar) {
+  if constexpr (C > 1)
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.multicast::cluster::all.b128 [%0], [%1];"
+                 ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+  else
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+// First CTA of the cluster whose launch was cancelled, or -1: there was none left.
+__device__ __forceinline__ int granted_cta(const uint4* answer) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=&r"(got), "=&r"(x) : "r"(smem_u32(answer)) : "memory");     // written before the address is read
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // read before the next answer may land here
+  return got ? static_cast<int>(x) : -1;
+}
+
 // Where the granules of this CTA's slice of a row are: [gs, ge) are whole; the row's elements before its first and behind
 // its last whole granule (fewer than n each) are `edge` elements, one for a thread of its own each.
 template <typename T>
@@ -458,6 +485,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
   __shared__ RowBars bars;
   __shared__ float2 part[2][C * kRowWarps];
   __shared__ EntryHead head[2];
+  __shared__ __align__(16) uint4 answer[4];
   __shared__ volatile int failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = C > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -475,6 +503,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
       mbar_init(&bars.e_empty[i], kRowWarps);
       mbar_init(&bars.xchg[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&bars.claim[i], 1);
     failed = 0;
     fence_barrier_init();
   }
@@ -488,19 +517,43 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
     cluster_wait();
   }
 
+  // The rows of this cluster: number 0 is its own; number i > 0 is requested after the exchange of row i - 2, when every
+  // warp of every CTA has read the answers up to i - 2, of which four are kept: number i in place (i - 1) % 4, the
+  // (i - 1) / 4-th answer there.  No request follows a refused one.
+  auto request = [&](int i) {              // by one thread of each CTA
+    const int at = (i - 1) & 3;
+    mbar_arrive_expect_tx(&bars.claim[at], 16);
+    if (rank == 0) request_row<C>(&answer[at], &bars.claim[at]);
+  };
+  auto answered = [&](int i) { return mbar_wait_soon(&bars.claim[(i - 1) & 3], ((i - 1) >> 2) & 1); };
+  auto granted = [&](int i) { return granted_cta(&answer[(i - 1) & 3]); };
+  auto next_row = [&](int i, long long& row) {     // by whole warps; every role asks for every number
+    const bool ok = warp < kRowWarps ? answered(i) : mbar_wait_idle(&bars.claim[(i - 1) & 3], ((i - 1) >> 2) & 1, 100);
+    if (!__all_sync(0xffffffffu, ok)) {
+      report_error(p.status, kErrProducerWait);
+      failed = 1;
+      return false;
+    }
+    const int cta = granted(i);
+    row = cta / C;
+    return cta >= 0 && row < p.T;
+  };
+  if (threadIdx.x == 0) request(1);
+
   if (warp == kRowWarps) {
     // ---------------------------------------------------------------- producer
-    if (lane == 0) {
-      int slot = 0;
-      uint32_t lap = 0;                    // parity of the ring's passes
-      bool ok = true;
-      for (int row = first_row; row < p.T && ok; row += plan.clusters) {
-        const T* src = static_cast<const T*>(p.logits) + row * p.ld;
-        const Granules<T> gr(src, p.V);
-        const Slice<T> sl(gr, rank, plan.per, p.V);
-        for (int k = 0; k < plan.chunks; ++k) {
-          ok = !failed && mbar_wait_idle(&bars.empty[slot], lap ^ 1, 100);
-          if (!ok) { report_error(p.status, kErrProducerWait); failed = 1; break; }
+    int slot = 0;
+    uint32_t lap = 0;                      // parity of the ring's passes
+    bool ok = true, more = true;
+    long long row = first_row;
+    for (int i = 1; ok && more; more = ok && next_row(i++, row)) {
+      const T* src = static_cast<const T*>(p.logits) + row * p.ld;
+      const Granules<T> gr(src, p.V);
+      const Slice<T> sl(gr, rank, plan.per, p.V);
+      for (int k = 0; k < plan.chunks; ++k) {
+        ok = __all_sync(0xffffffffu, !failed && mbar_wait_idle(&bars.empty[slot], lap ^ 1, 100));
+        if (!ok) { report_error(p.status, kErrProducerWait); failed = 1; break; }
+        if (lane == 0) {
           const int k0 = sl.g0 + k * kChunk, a = max(k0, sl.gs), b = min(k0 + kChunk, sl.ge);
           if (b > a) {
             const uint32_t bytes = static_cast<uint32_t>(b - a) * 16;
@@ -510,8 +563,8 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           } else {
             mbar_arrive(&bars.full[slot]);
           }
-          if (++slot == plan.ring) { slot = 0; lap ^= 1; }
         }
+        if (++slot == plan.ring) { slot = 0; lap ^= 1; }
       }
     }
   } else if (warp > kRowWarps) {
@@ -523,7 +576,10 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
     uint32_t* bitmap = reinterpret_cast<uint32_t*>(entry_base + 2 * entry_bytes(plan.kpad) + b * bitmap_bytes(plan.per, n));
     EntryHead& hd = head[b];
     uint32_t phase = 0;
-    for (long long row = first_row + static_cast<long long>(b) * plan.clusters; row < p.T; row += 2ll * plan.clusters, phase ^= 1) {
+    long long row = first_row;
+    bool more = true;
+    for (int number = 0; more; more = next_row(++number, row)) {
+      if ((number & 1) != b) continue;
       const T* src = static_cast<const T*>(p.logits) + row * p.ld;
       const Granules<T> gr(src, p.V);
       const int e0 = rank * plan.per * n - gr.lead, e1 = e0 + plan.per * n;
@@ -636,6 +692,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           if (!(gq[j] < 0.f)) Lane<TO>::store(dst + oid[j], (ex2(fmaf(os[j], c, -top)) * rs - gq[j]) * gw);
       }
       __syncwarp();
+      phase ^= 1;
     }
   } else {
     // ---------------------------------------------------------------- compute
@@ -644,7 +701,8 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
     const uint64_t c2 = pair(c, c);
     int it = 0, slot1 = 0, slot2 = 0;      // ring positions of the two passes
     uint32_t lap = 0;
-    for (long long row = first_row; row < p.T; row += plan.clusters, ++it) {
+    long long row = first_row;
+    for (bool more = true; more; more = next_row(++it, row)) {
       const int b = it & 1;
       const uint32_t phase = (it >> 1) & 1;
       const T* src = static_cast<const T*>(p.logits) + row * p.ld;
@@ -727,6 +785,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
       if (threadIdx.x == 0) {
         head[b].top = top;
         head[b].sum = sum;
+        if (answered(it + 1) && granted(it + 1) >= 0) request(it + 2);
       }
       if (p.grad != nullptr) {
         TO* dst = static_cast<TO*>(p.grad) + row * p.ldg;
@@ -971,15 +1030,15 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  // the shared-memory limit is raised once per device; how many clusters run at a time is asked once per size
+  // the shared-memory limit is raised once per device
   static std::atomic<unsigned long long> raised{0};
-  static std::atomic<unsigned long long> resident{0};      // device + 1, shared memory, clusters of the last question
   if (dev >= 64 || !((raised.load() >> dev) & 1ull)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
     if (e != cudaSuccess) return e;
     if (dev < 64) raised.fetch_or(1ull << dev);
   }
   cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.T) * C);
   cfg.blockDim = dim3(kRowThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -989,21 +1048,6 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const unsigned long long key = (static_cast<unsigned long long>(dev + 1) << 48) | (static_cast<unsigned long long>(smem) << 16);
-  unsigned long long known = resident.load();
-  if ((known & ~0xFFFFull) != key) {
-    int most = 0;
-    cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / C * C));
-    e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
-    if (e != cudaSuccess) return e;
-    known = key | static_cast<unsigned long long>(most < 1 ? 1 : most);
-    resident.store(known);
-  }
-  const int most = static_cast<int>(known & 0xFFFFull);
-  // whole rounds: with 1.2 rows per cluster every cluster takes two all the same
-  const int rounds = (p.T + most - 1) / most;
-  plan.clusters = (p.T + rounds - 1) / rounds;
-  cfg.gridDim = dim3(static_cast<unsigned>(plan.clusters) * C);
   return cudaLaunchKernelEx(&cfg, kernel, p, plan);
 }
 

@@ -298,6 +298,30 @@ def test_autograd_kernels_follow_the_definition(T, V, K, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,T,V", [(torch.bfloat16, 1501, 2001), (torch.float32, 999, 501), (torch.bfloat16, 401, 60000),
+                                       (torch.float32, 333, 50257), (torch.float32, 150, 151936)])
+def test_more_rows_than_run_at_a_time(dtype, T, V):
+    """Running clusters take over the rows of clusters that have not started: with 1, 2, 4 and 8 CTAs each."""
+    from steptronoss_b200.ops import native, topk_distillation, topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(T, V, 9, seed=9, dtype=dtype, device="cuda")
+    teacher[::7, 4:] = -INF
+    teacher[::11] = -INF
+    ids[::5, 1] = ids[::5, 0]
+    want, wgrad, p, q = oracle(logits, ids, teacher, 1.0, weights=w)
+    loss_tol, grad_tol = bounds(logits.cpu(), teacher.cpu(), 1.0, p, q, wgrad, w.double().cpu(), dtype)
+    for _ in range(3):
+        loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+        torch.cuda.synchronize()
+        native.raise_if_kernel_error()
+        assert (loss.double().cpu() - want).abs().max() <= loss_tol
+        assert ((grad.double().cpu() - wgrad).abs() <= grad_tol).all()
+    assert torch.equal(topk_distillation(logits, ids, teacher), loss)
+    buf = logits.clone()
+    assert torch.equal(topk_distillation_loss_and_grad(buf, ids, teacher, w, out=buf)[0], loss) and torch.equal(buf, grad)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_masks_repeated_and_foreign_ids_on_the_gpu(dtype):
     from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
