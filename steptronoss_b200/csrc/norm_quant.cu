@@ -68,42 +68,74 @@ __device__ __forceinline__ void scale_from_max(uint32_t bits, float steps, float
   else { scale = __fdiv_rn(amax, steps); inv = __fdiv_rn(steps, amax); }
 }
 
-// 8 columns starting at c of one bf16 row; columns from H on read as zero.
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int c, int H) {
-  if constexpr (VEC) {
-    return *reinterpret_cast<const uint4*>(row + c);
+// How a thread's i-th eight columns lie and are accessed:
+//   kVec    eight neighbouring columns in one access; every row starts on a 16-byte boundary, H is a multiple of 8
+//   kPair   four pairs, neighbouring threads side by side in each, 4 bytes per access; rows start on 4-byte boundaries, H
+//           is even
+//   kSingle the same pairs, element by element
+//   kBlock  eight neighbouring columns element by element (e4m3 blocks in rows on any address)
+// (515 x 1990: 8.6 us with eight neighbouring columns element by element, 3.6 us with pairs.)
+enum Access { kVec, kPair, kSingle, kBlock };
+
+template <Access A, int TPR>
+__device__ __forceinline__ int column(int tid, int i, int j) {     // of pair j
+  return A == kVec || A == kBlock ? 8 * (tid + i * TPR) + 2 * j : 2 * (tid + (4 * i + j) * TPR);
+}
+// Columns from H on read as zero.
+template <Access A, int TPR>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int tid, int i, int H) {
+  if constexpr (A == kVec) {
+    const int c = column<A, TPR>(tid, i, 0);
+    return c < H ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
   } else {
     const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
     uint32_t u[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int a = c + 2 * j;
-      u[j] = (a < H ? r[a] : 0u) | (a + 1 < H ? static_cast<uint32_t>(r[a + 1]) << 16 : 0u);
+      const int c = column<A, TPR>(tid, i, j);
+      if constexpr (A == kPair) u[j] = c < H ? *reinterpret_cast<const uint32_t*>(r + c) : 0u;
+      else u[j] = (c < H ? r[c] : 0u) | (c + 1 < H ? static_cast<uint32_t>(r[c + 1]) << 16 : 0u);
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void store8(__nv_bfloat16* row, int c, int H, const uint4& v) {
-  if constexpr (VEC) {
-    *reinterpret_cast<uint4*>(row + c) = v;
+template <Access A, int TPR>
+__device__ __forceinline__ void store8(__nv_bfloat16* row, int tid, int i, int H, const uint4& v) {
+  if constexpr (A == kVec) {
+    const int c = column<A, TPR>(tid, i, 0);
+    if (c < H) *reinterpret_cast<uint4*>(row + c) = v;
   } else {
     uint16_t* r = reinterpret_cast<uint16_t*>(row);
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < H) r[c + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+    for (int j = 0; j < 4; ++j) {
+      const int c = column<A, TPR>(tid, i, j);
+      if constexpr (A == kPair) {
+        if (c < H) *reinterpret_cast<uint32_t*>(r + c) = u[j];
+      } else {
+        if (c < H) r[c] = static_cast<uint16_t>(u[j]);
+        if (c + 1 < H) r[c + 1] = static_cast<uint16_t>(u[j] >> 16);
+      }
+    }
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void store8_bytes(uint8_t* row, int c, int H, uint32_t lo, uint32_t hi) {
-  if constexpr (VEC) {
-    *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+template <Access A, int TPR>
+__device__ __forceinline__ void store8_bytes(uint8_t* row, int tid, int i, int H, uint32_t lo, uint32_t hi) {
+  if constexpr (A == kVec) {
+    const int c = column<A, TPR>(tid, i, 0);
+    if (c < H) *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < H) row[c + j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    for (int j = 0; j < 4; ++j) {
+      const int c = column<A, TPR>(tid, i, j);
+      const uint32_t b = (j < 2 ? lo : hi) >> (16 * (j & 1));
+      if constexpr (A == kPair) {
+        if (c < H) *reinterpret_cast<uint16_t*>(row + c) = static_cast<uint16_t>(b);
+      } else {
+        if (c < H) row[c] = static_cast<uint8_t>(b);
+        if (c + 1 < H) row[c + 1] = static_cast<uint8_t>(b >> 8);
+      }
+    }
   }
 }
 
@@ -112,9 +144,8 @@ __device__ __forceinline__ void widen8(const uint4& u, float (&f)[8]) {
   f[4] = bf16_lo(u.z); f[5] = bf16_hi(u.z); f[6] = bf16_lo(u.w); f[7] = bf16_hi(u.w);
 }
 
-// TPR threads share a row (a whole CTA, or one of the CTA's four warps when TPR is 32); NV vectors per thread.
-// VEC: every row starts on a 16-byte boundary and H is a multiple of 8; otherwise element by element.
-template <int TPR, int NV, bool E4M3, bool VEC>
+// TPR threads share a row (a whole CTA, or one of the CTA's four warps when TPR is 32); NV times 8 columns per thread.
+template <int TPR, int NV, bool E4M3, Access A>
 __global__ void __launch_bounds__(TPR < 128 ? (TPR == 32 ? 128 : TPR) : TPR)
 norm_quant_kernel(const NormQuantParams p) {
   __shared__ float red_sum[32];
@@ -124,22 +155,18 @@ norm_quant_kernel(const NormQuantParams p) {
   if (TPR == 32 && row >= p.rows) return;     // whole warps leave, and no block barrier follows
   const __nv_bfloat16* xr = p.x + row * p.ldx;
   const __nv_bfloat16* dr = p.delta != nullptr ? p.delta + row * p.ldd : nullptr;
-  const int nvec = (p.H + 7) / 8;
 
   uint4 v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int k = tid + i * TPR;
-    v[i] = k < nvec ? load8<VEC>(xr, k * 8, p.H) : make_uint4(0, 0, 0, 0);
+    v[i] = load8<A, TPR>(xr, tid, i, p.H);
   }
   if (dr != nullptr) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int k = tid + i * TPR;
-      if (k >= nvec) continue;
       float a[8], b[8];
       widen8(v[i], a);
-      widen8(load8<VEC>(dr, k * 8, p.H), b);
+      widen8(load8<A, TPR>(dr, tid, i, p.H), b);
       v[i] = make_uint4(pack_bf16(a[0] + b[0], a[1] + b[1]), pack_bf16(a[2] + b[2], a[3] + b[3]),
                         pack_bf16(a[4] + b[4], a[5] + b[5]), pack_bf16(a[6] + b[6], a[7] + b[7]));
     }
@@ -147,8 +174,7 @@ norm_quant_kernel(const NormQuantParams p) {
   if (p.s != nullptr) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int k = tid + i * TPR;
-      if (k < nvec) store8<VEC>(p.s + row * p.lds, k * 8, p.H, v[i]);
+      store8<A, TPR>(p.s + row * p.lds, tid, i, p.H, v[i]);
     }
   }
   float rstd = 1.f;
@@ -169,9 +195,8 @@ norm_quant_kernel(const NormQuantParams p) {
   auto normed = [&](int i, float (&f)[8]) {
     widen8(v[i], f);
     if (p.w == nullptr) return;
-    const int k = tid + i * TPR;
     float g[8];
-    widen8(k < nvec ? load8<VEC>(p.w, k * 8, p.H) : make_uint4(0, 0, 0, 0), g);
+    widen8(load8<A, TPR>(p.w, tid, i, p.H), g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * (g[j] + woff);
   };
@@ -195,7 +220,7 @@ norm_quant_kernel(const NormQuantParams p) {
       for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
       float scale, inv;
       scale_from_max(m, 448.f, scale, inv);
-      if (k >= nvec) continue;
+      if (k * 8 >= p.H) continue;
       uint32_t out[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -203,14 +228,16 @@ norm_quant_kernel(const NormQuantParams p) {
         const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h + 2] * inv, f[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
         out[h] = a | (b << 16);
       }
-      store8_bytes<VEC>(qr, k * 8, p.H, out[0], out[1]);
+      store8_bytes<A, TPR>(qr, tid, i, p.H, out[0], out[1]);
       if ((k & 15) == 0) p.scale[row * kbs + (k >> 4)] = scale;
     }
   } else {
+    constexpr bool kKeep = NV <= 2;            // y stays in registers where it is small
+    float y[kKeep ? NV : 1][8];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float f[8];
+      float (&f)[8] = y[kKeep ? i : 0];
       normed(i, f);
       m = max(m, top_of(f));
     }
@@ -220,42 +247,40 @@ norm_quant_kernel(const NormQuantParams p) {
     if (tid == 0) p.scale[row] = scale;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int k = tid + i * TPR;
-      if (k >= nvec) continue;
-      float f[8];
-      normed(i, f);
+      float (&f)[8] = y[kKeep ? i : 0];
+      if constexpr (!kKeep) normed(i, f);
       uint32_t out[2] = {0u, 0u};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         // |y * inv| <= 127 up to rounding, or y * 0 for the rows without a scale (NaN converts to 0)
         out[j >> 2] |= (static_cast<uint32_t>(__float2int_rn(f[j] * inv)) & 0xFFu) << (8 * (j & 3));
       }
-      store8_bytes<VEC>(qr, k * 8, p.H, out[0], out[1]);
+      store8_bytes<A, TPR>(qr, tid, i, p.H, out[0], out[1]);
     }
   }
 }
 
-template <int TPR, bool E4M3, bool VEC>
+template <int TPR, bool E4M3, Access A>
 static cudaError_t launch_norm_quant(const NormQuantParams& p, int nv, cudaStream_t stream) {
   const int threads = TPR == 32 ? 128 : TPR;
   const long long blocks = TPR == 32 ? (p.rows + 3) / 4 : p.rows;
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (nv <= 1) norm_quant_kernel<TPR, 1, E4M3, VEC><<<grid, threads, 0, stream>>>(p);
-  else if (nv <= 2) norm_quant_kernel<TPR, 2, E4M3, VEC><<<grid, threads, 0, stream>>>(p);
-  else norm_quant_kernel<TPR, 4, E4M3, VEC><<<grid, threads, 0, stream>>>(p);
+  if (nv <= 1) norm_quant_kernel<TPR, 1, E4M3, A><<<grid, threads, 0, stream>>>(p);
+  else if (nv <= 2) norm_quant_kernel<TPR, 2, E4M3, A><<<grid, threads, 0, stream>>>(p);
+  else norm_quant_kernel<TPR, 4, E4M3, A><<<grid, threads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
-template <bool E4M3, bool VEC>
+template <bool E4M3, Access A>
 static cudaError_t dispatch_norm_quant(const NormQuantParams& p, cudaStream_t stream) {
   // Threads per row: two vectors per thread, so that a row's loads are in flight together and an SM holds many rows.
   const int nvec = (p.H + 7) / 8;
-  if (nvec <= 64) return launch_norm_quant<32, E4M3, VEC>(p, (nvec + 31) / 32, stream);
-  if (nvec <= 128) return launch_norm_quant<64, E4M3, VEC>(p, 2, stream);
-  if (nvec <= 256) return launch_norm_quant<128, E4M3, VEC>(p, 2, stream);
-  if (nvec <= 512) return launch_norm_quant<256, E4M3, VEC>(p, 2, stream);
-  if (nvec <= 1024) return launch_norm_quant<512, E4M3, VEC>(p, 2, stream);
-  return launch_norm_quant<1024, E4M3, VEC>(p, (nvec + 1023) / 1024, stream);
+  if (nvec <= 64) return launch_norm_quant<32, E4M3, A>(p, (nvec + 31) / 32, stream);
+  if (nvec <= 128) return launch_norm_quant<64, E4M3, A>(p, 2, stream);
+  if (nvec <= 256) return launch_norm_quant<128, E4M3, A>(p, 2, stream);
+  if (nvec <= 512) return launch_norm_quant<256, E4M3, A>(p, 2, stream);
+  if (nvec <= 1024) return launch_norm_quant<512, E4M3, A>(p, 2, stream);
+  return launch_norm_quant<1024, E4M3, A>(p, (nvec + 1023) / 1024, stream);
 }
 
 }  // namespace stb
@@ -281,7 +306,11 @@ extern "C" int stb_norm_quant(const void* x, const void* delta, const void* w, v
   const bool vec = H % 8 == 0 && on16(x, ldx) && on16(delta, ldd) && on16(s, lds) && on16(w, 0) &&
                    reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
   cudaError_t e;
-  if (fmt == 1) e = vec ? dispatch_norm_quant<true, true>(p, stream) : dispatch_norm_quant<true, false>(p, stream);
-  else e = vec ? dispatch_norm_quant<false, true>(p, stream) : dispatch_norm_quant<false, false>(p, stream);
+  auto on4 = [](const void* t, long long ld) { return t == nullptr || (reinterpret_cast<uintptr_t>(t) % 4 == 0 && ld % 2 == 0); };
+  const bool pairs = H % 2 == 0 && on4(x, ldx) && on4(delta, ldd) && on4(s, lds) && on4(w, 0) &&
+                     reinterpret_cast<uintptr_t>(q) % 2 == 0 && ldq % 2 == 0;
+  if (fmt == 1) e = vec ? dispatch_norm_quant<true, kVec>(p, stream) : dispatch_norm_quant<true, kBlock>(p, stream);
+  else if (vec) e = dispatch_norm_quant<false, kVec>(p, stream);
+  else e = pairs ? dispatch_norm_quant<false, kPair>(p, stream) : dispatch_norm_quant<false, kSingle>(p, stream);
   return -static_cast<int>(e);
 }

@@ -64,14 +64,20 @@ def _checked(rows: int, index: int, teacher_ids, teacher_logits, temperature, wh
     if teacher_ids.get_device() != index or teacher_logits.get_device() != index:
         raise ValueError(f"{what}: teacher entries on {teacher_ids.device} / {teacher_logits.device}, not on the student's "
                          "device")
-    if not (temperature > 0.0 and math.isfinite(temperature) and math.isfinite(1.0 / temperature)):
-        raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{what}: temperature must lie between 1e-6 and 1e6, got {temperature}")
     if len(shape) != 2:
         teacher_ids, teacher_logits = teacher_ids.reshape(rows, K), teacher_logits.reshape(rows, K)
     if teacher_logits.dtype != torch.float32:
         teacher_logits = teacher_logits.float()
     return (teacher_ids if teacher_ids.stride(1) == 1 else teacher_ids.contiguous(),
             teacher_logits if teacher_logits.stride(1) == 1 else teacher_logits.contiguous())
+
+
+def _check_shard(V: int, vocab_start: int, group, what: str) -> None:
+    if not 0 <= vocab_start <= V * (_group_size(group) - 1):
+        raise ValueError(f"{what}: a shard of {V} from {vocab_start} on does not lie in a vocabulary of {_group_size(group)} "
+                         "such shards")
 
 
 def _rows_of(logits: torch.Tensor, what: str) -> torch.Tensor:
@@ -265,10 +271,11 @@ def topk_distillation(logits, teacher_ids, teacher_logits, temperature: float = 
 
     ``logits`` may be a vocabulary shard of equal size on every rank of ``group``, starting at ``vocab_start``;
     ``teacher_ids`` are always ids of the whole vocabulary.  Differentiable with respect to ``logits``."""
-    temperature = float(temperature)
+    temperature, vocab_start = float(temperature), int(vocab_start)
     rows = math.prod(logits.shape[:-1])
+    _check_shard(logits.shape[-1] if logits.dim() else 0, vocab_start, group, "topk_distillation")
     ids, t = _checked(rows, logits.get_device(), teacher_ids, teacher_logits, temperature, "topk_distillation")
-    return _TopkDistillationFn.apply(logits, ids, t, temperature, int(vocab_start), group)
+    return _TopkDistillationFn.apply(logits, ids, t, temperature, vocab_start, group)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -413,6 +420,7 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
         raise ValueError(f"{what}: h is [T, H] and w [V, H], got {tuple(h.shape)} and {tuple(w.shape)}")
     if chunk_tokens < 1:
         raise ValueError(f"{what}: chunk_tokens must be positive, got {chunk_tokens}")
+    _check_shard(w.shape[0], int(vocab_start), group, what)
     if w.device != h.device:
         raise ValueError(f"{what}: h on {h.device}, w on {w.device}")
     ids, t = _checked(h.shape[0], h.get_device(), teacher_ids, teacher_logits, temperature, what)

@@ -94,10 +94,14 @@ def gemm_int8_reference(xq, sx, wq, sw, out_dtype: torch.dtype = torch.bfloat16)
     return (dot.float() * sx.unsqueeze(-1) * sw.unsqueeze(0)).to(out_dtype)
 
 
-def _rows_aligned(t: torch.Tensor) -> bool:
+def _pitch(t: torch.Tensor) -> int:
+    """Bytes from row to row if the kernel takes these rows, else 0 (a single row has any pitch)."""
     pitch, step = t.stride()
     rows, width = t.shape
-    return t.data_ptr() % 16 == 0 and pitch % 16 == 0 and pitch >= width and (step == 1 or width == 1) or rows == 0
+    if rows <= 1:
+        pitch = (width + 15) // 16 * 16
+    ok = t.data_ptr() % 16 == 0 and pitch % 16 == 0 and pitch >= width and (step == 1 or width == 1)
+    return pitch if ok or rows == 0 else 0
 
 
 def gemm_int8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor,
@@ -131,7 +135,8 @@ def gemm_int8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
     if index < 0:
         res = gemm_int8_reference(xq, sx, wq, sw, out_dtype)
         return res if out is None else out.copy_(res)
-    if not _rows_aligned(xq) or not _rows_aligned(wq):
+    ldx, ldw = _pitch(xq), _pitch(wq)
+    if not ldx or not ldw:
         raise ValueError(f"gemm_int8: the rows of xq and wq must be contiguous and start on 16-byte boundaries, got "
                          f"strides {xq.stride()} and {wq.stride()} (quantize_rows_int8 returns such rows, pitched_like "
                          "makes them)")
@@ -144,7 +149,7 @@ def gemm_int8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
         if not sw.is_contiguous():
             sw = sw.contiguous()
         rc = native.launch(native.load().stb_gemm_int8, index, xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(),
-                           out.data_ptr(), M, N, K, xq.stride(0), wq.stride(0), out.stride(0) if M > 1 else N,
+                           out.data_ptr(), M, N, K, ldx, ldw, out.stride(0) if M > 1 else N,
                            int(out_dtype == torch.float32), native.status_ptr(index))
         if rc:
             native.check(rc, f"gemm_int8 M={M} N={N} K={K}")

@@ -173,6 +173,8 @@ def test_fused_head_on_cpu_is_the_head_and_the_loss():
     (dict(temperature=-1.0), ValueError),
     (dict(temperature=math.nan), ValueError),
     (dict(temperature=math.inf), ValueError),
+    (dict(temperature=1e-7), ValueError),
+    (dict(temperature=1e7), ValueError),
     (dict(weights=torch.ones(3)), ValueError),
     (dict(logits=torch.zeros(2, 2, 9)), ValueError),
     (dict(logits=torch.zeros(4, 0)), ValueError),
@@ -199,6 +201,26 @@ def test_refuses_an_output_that_overlaps_the_logits():
     logits, out = buf[:36].view(4, 9), buf[4:40].view(4, 9)
     with pytest.raises(ValueError):
         topk_distillation_loss_and_grad(logits, torch.zeros(4, 2, dtype=torch.long), torch.zeros(4, 2), torch.ones(4), out=out)
+
+
+def test_refuses_a_shard_outside_the_vocabulary():
+    from steptronoss_b200.ops import fused_linear_topk_distillation, topk_distillation
+
+    ids, t = torch.zeros(4, 2, dtype=torch.long), torch.zeros(4, 2)
+    for start in (-1, 1, 9):
+        with pytest.raises(ValueError):
+            topk_distillation(torch.zeros(4, 9), ids, t, 1.0, start)
+        with pytest.raises(ValueError):
+            fused_linear_topk_distillation(torch.zeros(4, 8), torch.zeros(16, 8), ids, t, torch.ones(4), 1.0, start)
+
+
+def test_second_derivatives_are_refused():
+    from steptronoss_b200.ops import topk_distillation
+
+    logits, ids, teacher, _ = make(3, 9, 2)
+    loss = topk_distillation(logits.requires_grad_(), ids, teacher).sum()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, logits, create_graph=True)
 
 
 def test_fused_head_refusals():
@@ -431,6 +453,41 @@ def test_rows_longer_than_a_cluster_holds(dtype, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_longest_row_of_the_one_pass_kernel_with_the_most_entries(dtype):
+    from steptronoss_b200.ops import native, topk_distillation_loss_and_grad
+
+    V = native.load().stb_distill_row_limit(dtype.itemsize)
+    logits, ids, teacher, w = make(1, V, 1024, seed=10, dtype=dtype, device="cuda")
+    ids[0, 3], ids[0, 4] = V - 1, 0
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    torch.cuda.synchronize()
+    native.raise_if_kernel_error()
+    check(loss, grad, logits, ids, teacher, w, 1.0)
+
+
+@pytest.mark.gpu
+def test_more_elements_than_32_bits_count():
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    T, V, K, last = 14200, 151936, 8, 3
+    assert T * V > 2 ** 31
+    tail, ids, teacher, w = make(last, V, K, seed=11, dtype=torch.bfloat16, device="cuda")
+    logits = torch.zeros(T, V, dtype=torch.bfloat16, device="cuda")
+    logits[-last:] = tail
+    all_ids = torch.zeros(T, K, dtype=torch.int64, device="cuda")
+    all_t = torch.full((T, K), -INF, device="cuda")
+    all_w = torch.ones(T, device="cuda")
+    all_ids[-last:], all_t[-last:], all_w[-last:] = ids, teacher, w
+    stats_loss = topk_distillation(logits, all_ids, all_t)
+    x = logits[-last:].clone().requires_grad_()
+    loss, grad = topk_distillation_loss_and_grad(logits, all_ids, all_t, all_w, out=logits)
+    assert torch.equal(loss, stats_loss) and loss[:-last].eq(0).all()
+    check(loss[-last:], grad[-last:], tail, ids, teacher, w, 1.0)
+    assert not grad[:-last].any()
+
+
+@pytest.mark.gpu
 def test_many_entries():
     from steptronoss_b200.ops import topk_distillation_loss_and_grad
 
@@ -514,6 +571,18 @@ def test_fused_head_follows_the_definition(T, H, V, chunk):
     with torch.no_grad():
         total2, tok2 = fused_linear_topk_distillation(h, head, ids, teacher, w, tau, chunk_tokens=chunk)
     assert torch.equal(tok, tok2) and total2 == total
+
+
+@pytest.mark.gpu
+def test_fused_head_without_tokens():
+    from steptronoss_b200.ops import fused_linear_topk_distillation
+
+    _, ids, teacher, w = make(3, 64, 2, device="cuda")
+    h = torch.zeros(0, 16, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    head = torch.zeros(64, 16, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    total, tok = fused_linear_topk_distillation(h, head, ids[:0], teacher[:0], w[:0])
+    dh, dw = torch.autograd.grad(total, [h, head])
+    assert total == 0 and tok.shape == (0,) and dh.shape == (0, 16) and dw.eq(0).all()
 
 
 @pytest.mark.gpu

@@ -152,6 +152,30 @@ def test_rows_behind_the_last_token_stay():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(20000, 110000), (129, 17000000)])
+def test_more_results_than_32_bits_count(M, N):
+    from steptronoss_b200 import ops
+
+    assert M * N > 2 ** 31
+    xq, sx, wq, sw = operands(M, 64, 32, "cuda")
+    wq, sw = wq.repeat((N + 63) // 64, 1)[:N], sw.repeat((N + 63) // 64)[:N].contiguous()
+    y = ops.gemm_int8(xq, sx, wq, sw)
+    for rows in (slice(0, 2), slice(M - 2, M)):
+        for cols in (slice(0, 200), slice(N - 200, N)):
+            check(y[rows, cols], xq[rows], sx[rows], wq[cols], sw[cols])
+
+
+@pytest.mark.gpu
+def test_a_single_row_needs_no_pitch():
+    from steptronoss_b200 import ops
+
+    xq, sx, wq, sw = operands(1, 300, 100, "cuda")
+    flat = torch.empty(1, 100, dtype=torch.int8, device="cuda").copy_(xq)
+    assert flat.stride(0) == 100
+    check(ops.gemm_int8(flat, sx, wq, sw), xq, sx, wq, sw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M,K", [(1, 1), (1, 8), (3, 7), (300, 128), (5, 1990), (77, 2050), (9, 4096), (4, 12288), (2, 32768),
                                  (3, 20001)])
 def test_quantised_rows(M, K):
