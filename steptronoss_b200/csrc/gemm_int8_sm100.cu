@@ -317,7 +317,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         } else {
           // rows on any address: the group's 128 channels of a token lie side by side in shared memory and leave as
           // 16-byte stores from the first 16-byte boundary on, what is before and behind them element by element.  (With
-          // one 2-byte store per channel 1333 x 5001 x 2050 took 42 us instead of XXX.)
+          // one 2-byte store per channel 1333 x 5001 x 2050 took 42 us instead of 27.)
           __nv_bfloat16* buf = group_stage + (stores++ & 1) * (32 * 128);
           __nv_bfloat16* out = buf + quarter * 32 + lane;
 #pragma unroll
