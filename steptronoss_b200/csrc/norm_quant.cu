@@ -47,25 +47,66 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   }
   return v;
 }
+// The bits of non-negative floats, NaN included, are ordered like integers.
 template <int TPR>
-__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
-  v = __reduce_max_sync(0xffffffffu, v);
+__device__ __forceinline__ float row_max(float top, uint32_t* red) {
+  uint32_t v = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   if constexpr (TPR > 32) {
     const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
     if (l == 0) red[w] = v;
     __syncthreads();
     v = __reduce_max_sync(0xffffffffu, l < TPR / 32 ? red[l] : 0u);
   }
-  return v;
+  return __uint_as_float(v);
 }
 
-// Scale and its inverse from the bits of max|y| (compared as integers: NaN is above infinity, which is above every
-// number).  Below 6e-36 max / 448 leaves the range of normal numbers; such values count as zero.
-__device__ __forceinline__ void scale_from_max(uint32_t bits, float steps, float& scale, float& inv) {
-  const float amax = __uint_as_float(bits);
-  if (bits >= 0x7F800000u) { scale = __uint_as_float(0x7FC00000u); inv = 0.f; }
-  else if (amax < 6e-36f) { scale = 1.f; inv = 0.f; }
-  else { scale = __fdiv_rn(amax, steps); inv = __fdiv_rn(steps, amax); }
+// Largest |y| of eight values; a NaN stays one (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+// Whether max|y| gives a scale.  Below 6e-36 max / 448 leaves the range of normal numbers; such values count as zero.
+__device__ __forceinline__ bool usable(float amax) { return amax >= 6e-36f && amax < INFINITY; }
+__device__ __forceinline__ float scale_of(float amax, float steps) {
+  return usable(amax) ? __fdiv_rn(amax, steps) : amax < 6e-36f ? 1.f : __uint_as_float(0x7FC00000u);
+}
+// 1 / scale to within 2 units in the last place: it only decides between neighbouring 8-bit values at their border
+__device__ __forceinline__ float inverse_of(float amax, float steps) { return usable(amax) ? __fdividef(steps, amax) : 0.f; }
+
+// Two fp32 at once: one instruction on this architecture.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ void widen4x2(const uint4& u, uint64_t (&f)[4]) {
+  f[0] = pack2(bf16_lo(u.x), bf16_hi(u.x));
+  f[1] = pack2(bf16_lo(u.y), bf16_hi(u.y));
+  f[2] = pack2(bf16_lo(u.z), bf16_hi(u.z));
+  f[3] = pack2(bf16_lo(u.w), bf16_hi(u.w));
+}
+// bf16(a + b) of two pairs.  One rounding of the exact sum is what an fp32 addition followed by a rounding gives: the fp32
+// sum of two bf16 numbers is inexact only where one of them is too small to move the other at all.
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 s = __hadd2_rn(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&s);
 }
 
 // How a thread's i-th eight columns lie and are accessed:
@@ -139,11 +180,6 @@ __device__ __forceinline__ void store8_bytes(uint8_t* row, int tid, int i, int H
   }
 }
 
-__device__ __forceinline__ void widen8(const uint4& u, float (&f)[8]) {
-  f[0] = bf16_lo(u.x); f[1] = bf16_hi(u.x); f[2] = bf16_lo(u.y); f[3] = bf16_hi(u.y);
-  f[4] = bf16_lo(u.z); f[5] = bf16_hi(u.z); f[6] = bf16_lo(u.w); f[7] = bf16_hi(u.w);
-}
-
 // TPR threads share a row (a whole CTA, or one of the CTA's four warps when TPR is 32); NV times 8 columns per thread.
 template <int TPR, int NV, bool E4M3, Access A>
 __global__ void __launch_bounds__(TPR < 128 ? (TPR == 32 ? 128 : TPR) : TPR)
@@ -164,11 +200,8 @@ norm_quant_kernel(const NormQuantParams p) {
   if (dr != nullptr) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float a[8], b[8];
-      widen8(v[i], a);
-      widen8(load8<A, TPR>(dr, tid, i, p.H), b);
-      v[i] = make_uint4(pack_bf16(a[0] + b[0], a[1] + b[1]), pack_bf16(a[2] + b[2], a[3] + b[3]),
-                        pack_bf16(a[4] + b[4], a[5] + b[5]), pack_bf16(a[6] + b[6], a[7] + b[7]));
+      const uint4 d = load8<A, TPR>(dr, tid, i, p.H);
+      v[i] = make_uint4(add_bf16x2(v[i].x, d.x), add_bf16x2(v[i].y, d.y), add_bf16x2(v[i].z, d.z), add_bf16x2(v[i].w, d.w));
     }
   }
   if (p.s != nullptr) {
@@ -179,31 +212,40 @@ norm_quant_kernel(const NormQuantParams p) {
   }
   float rstd = 1.f;
   if (p.w != nullptr) {
-    float ss = 0.f;
+    uint64_t ss2 = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float f[8];
-      widen8(v[i], f);
+      uint64_t f[4];
+      widen4x2(v[i], f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
+      for (int j = 0; j < 4; ++j) ss2 = fma2(f[j], f[j], ss2);
     }
-    rstd = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(ss, red_sum), static_cast<float>(p.H)) + p.eps);
+    float a, b;
+    unpack2(ss2, a, b);
+    rstd = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(a + b, red_sum), static_cast<float>(p.H)) + p.eps);
   }
-  const float woff = p.zero_centered ? 1.f : 0.f;
 
-  // y of one vector, in fp32 (recomputed where it is needed twice: the registers hold the bf16 sum)
-  auto normed = [&](int i, float (&f)[8]) {
-    widen8(v[i], f);
+  // y of eight columns, in fp32 (recomputed where it is needed twice and not kept: the registers hold the bf16 sum)
+  auto normed = [&](int i, uint64_t (&f)[4]) {
+    widen4x2(v[i], f);
     if (p.w == nullptr) return;
-    float g[8];
-    widen8(load8<A, TPR>(p.w, tid, i, p.H), g);
+    uint64_t g[4];
+    widen4x2(load8<A, TPR>(p.w, tid, i, p.H), g);
+    if (p.zero_centered) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * (g[j] + woff);
+      for (int j = 0; j < 4; ++j) g[j] = add2(g[j], pack2(1.f, 1.f));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = mul2(mul2(f[j], pack2(rstd, rstd)), g[j]);
   };
-  auto top_of = [](const float (&f)[8]) {
-    uint32_t m = 0;
+  auto top_of = [](const uint64_t (&f)[4]) {
+    float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7FFFFFFFu);
+    for (int j = 0; j < 4; ++j) {
+      float a, b;
+      unpack2(f[j], a, b);
+      m = max_nan(m, max_nan(fabsf(a), fabsf(b)));
+    }
     return m;
   };
   uint8_t* qr = p.q + row * p.ldq;
@@ -213,47 +255,59 @@ norm_quant_kernel(const NormQuantParams p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int k = tid + i * TPR;
-      float f[8];
+      uint64_t f[4];
       normed(i, f);
-      uint32_t m = top_of(f);
+      float m = top_of(f);
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      float scale, inv;
-      scale_from_max(m, 448.f, scale, inv);
+      for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (k * 8 >= p.H) continue;
+      const float inv = inverse_of(m, 448.f);
       uint32_t out[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h] * inv, f[4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h + 2] * inv, f[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-        out[h] = a | (b << 16);
+        float a, b, c, d;
+        unpack2(mul2(f[2 * h], pack2(inv, inv)), a, b);
+        unpack2(mul2(f[2 * h + 1], pack2(inv, inv)), c, d);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+        out[h] = lo | (hi << 16);
       }
       store8_bytes<A, TPR>(qr, tid, i, p.H, out[0], out[1]);
-      if ((k & 15) == 0) p.scale[row * kbs + (k >> 4)] = scale;
+      if ((k & 15) == 0) p.scale[row * kbs + (k >> 4)] = scale_of(m, 448.f);
     }
   } else {
     constexpr bool kKeep = NV <= 2;            // y stays in registers where it is small
-    float y[kKeep ? NV : 1][8];
-    uint32_t m = 0;
+    uint64_t y[kKeep ? NV : 1][4];
+    float m = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float (&f)[8] = y[kKeep ? i : 0];
+      uint64_t (&f)[4] = y[kKeep ? i : 0];
       normed(i, f);
-      m = max(m, top_of(f));
+      m = max_nan(m, top_of(f));
     }
     m = row_max<TPR>(m, red_max);
-    float scale, inv;
-    scale_from_max(m, 127.f, scale, inv);
-    if (tid == 0) p.scale[row] = scale;
+    const float inv = inverse_of(m, 127.f);
+    if (tid == 0) p.scale[row] = scale_of(m, 127.f);
+    const bool some = usable(m);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float (&f)[8] = y[kKeep ? i : 0];
+      uint64_t (&f)[4] = y[kKeep ? i : 0];
       if constexpr (!kKeep) normed(i, f);
       uint32_t out[2] = {0u, 0u};
+      if (some) {                              // rows without a scale become zeros, whatever they hold
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // |y * inv| <= 127 up to rounding, or y * 0 for the rows without a scale (NaN converts to 0)
-        out[j >> 2] |= (static_cast<uint32_t>(__float2int_rn(f[j] * inv)) & 0xFFu) << (8 * (j & 3));
+        for (int h = 0; h < 2; ++h) {
+          // y * inv + 1.5 * 2^23 leaves the nearest integer (ties to even) in the low bits; |y * inv| <= 127 up to rounding
+          uint32_t r[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float a, b;
+            unpack2(fma2(f[2 * h + j], pack2(inv, inv), pack2(12582912.f, 12582912.f)), a, b);
+            r[2 * j] = __float_as_uint(a);
+            r[2 * j + 1] = __float_as_uint(b);
+          }
+          out[h] = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+        }
       }
       store8_bytes<A, TPR>(qr, tid, i, p.H, out[0], out[1]);
     }

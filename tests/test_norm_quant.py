@@ -91,6 +91,23 @@ def test_kernel_follows_the_definition(T, H):
 
 
 @pytest.mark.gpu
+def test_residual_sum_of_any_two_magnitudes_is_rounded_once():
+    from steptronoss_b200 import ops
+
+    torch.manual_seed(3)
+    T, H = 64, 4096
+    x, d = ((torch.randn(T, H, device="cuda") * torch.randint(-30, 31, (T, H), device="cuda").float().exp2()).to(torch.bfloat16)
+            for _ in range(2))
+    d[:, ::3] = -x[:, ::3] * 1.0078125                        # near cancellation
+    d[:, 1::7] = x[:, 1::7] * 2.0 ** -9                       # ties of the sum's last place
+    w = torch.ones(H, dtype=torch.bfloat16, device="cuda")
+    want = (x.double() + d.double()).to(torch.float32).to(torch.bfloat16)
+    for fmt in ("int8", "e4m3_1x128"):
+        s, _, _ = ops.add_rmsnorm_quant(x, d, w, fmt=fmt)
+        assert torch.equal(s, want) and torch.equal(s, ops.add_rmsnorm(x, d, w)[0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["int8", "e4m3_1x128"])
 def test_strides_alignment_and_rows_without_numbers(fmt):
     from steptronoss_b200 import ops
