@@ -24,7 +24,7 @@
 
 namespace stb {
 
-constexpr int kDsThreads = 256;
+constexpr int kDsThreads = 256;              // gradient kernel
 constexpr int kDsMaxEntries = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -163,7 +163,7 @@ __device__ __forceinline__ void warp_merge(float& m, float& s) {
   m = top;
 }
 
-// Teacher entries of a row in shared memory, filled by warp 0.
+// Teacher entries of a row in shared memory (statistics and gradient kernels).
 struct Entries {
   float q[kDsMaxEntries];      // probability, 0 where there is no entry
   float s[kDsMaxEntries];      // the student's logit there (0 where the id is not in this shard)
@@ -226,16 +226,15 @@ __device__ __forceinline__ float warp_total(float v) {
   return v;
 }
 
-// Gradient at the ids that `mine(local id)` says are this CTA's: written once more over the dense p, from the logit
-// kept in shared memory, with the q of equal ids added in order.  The caller has a barrier between the dense writes
-// and this.
-template <typename TO, typename Mine>
+// Gradient at the entries: written once more over the dense p, from the logit kept in shared memory, with the q of equal
+// ids added in order.  The caller has a barrier between the dense writes and this.
+template <typename TO>
 __device__ __forceinline__ void write_entries(const DistillParams& p, const Entries& e, TO* grad_row, const float4& st,
-                                              float w, Mine mine) {
+                                              float w) {
   const float c = p.inv_tau * kLog2e, g = w * p.inv_tau, inv = __fdiv_rn(1.f, st.y);
   for (int j = threadIdx.x; j < p.K; j += blockDim.x) {
     const int id = e.id[j];
-    if (id < 0 || !mine(id)) continue;
+    if (id < 0) continue;
     bool first = true;
     float q = 0.f;
     for (int i = 0; i < p.K; ++i) {
@@ -286,7 +285,12 @@ __device__ __forceinline__ void block_merge(float& m, float& s, float2* red) {
 //                   memory, straight to global memory
 //
 // Loads, entries and the cluster's exchange thus run beside the arithmetic; nothing waits for the whole CTA.
-// Bound: DRAM for fp32 logits; for bf16 the exponentials (two per element, 16 a cycle and SM) come close to it.
+//
+// Bound: DRAM for fp32 logits (2048 x 151936: 397 us, 6.27 TB/s of 6.55 measured).  For bf16 the exponentials (two per
+// element, 16 a cycle and SM: 277 us of 4096 x 151936) and the issue slots (15 per element, half of them for what a row costs
+// a warp whatever its length) are both busy for about 60 % of the time: 471 us, 5.3 TB/s.  Measured around this point, same
+// size: 4, 6 or 12 compute warps 554, 588, 480 us; 3 or 4 smaller CTAs on an SM 513-570; two or eight granules per thread and
+// chunk 553, 580; every fourth exponential by a polynomial instead of the special-function unit 522 against 524 at the time.
 constexpr int kU = 4;                            // granules per compute thread and chunk
 constexpr int kRowWarps = 8;                     // compute warps
 constexpr int kRowCompute = 32 * kRowWarps;
@@ -964,7 +968,7 @@ distill_grad_kernel(const DistillParams p, int chunks) {
   }
   if (zero) return;
   __syncthreads();
-  write_entries<TO>(p, e, dst, st, w, [](int) { return true; });
+  write_entries<TO>(p, e, dst, st, w);
 }
 
 // ------------------------------------------------------------------------------------------- fused head: total, scaling
@@ -1081,7 +1085,7 @@ extern "C" int stb_distill_row_limit(int elem_bytes) {
 }
 
 static bool distill_args_ok(const DistillParams& p) {
-  return p.T > 0 && p.T <= 0x0FFFFFFF && p.V > 0 && p.K >= 0 && p.K <= kDsMaxEntries && p.inv_tau > 0.f;
+  return p.T > 0 && p.T <= 0x0FFFFFFF && p.V > 0 && p.V <= (1 << 30) && p.K >= 0 && p.K <= kDsMaxEntries && p.inv_tau > 0.f;
 }
 
 // The gradient has the logits' type, or is bf16 for fp32 logits.

@@ -100,12 +100,13 @@ def _token_weights(weights, rows: int, index: int, what: str) -> torch.Tensor:
 # --------------------------------------------------------------------------------------------------- PyTorch statement
 def _teacher_q(ids, t, temperature: float, vocab: int):
     """``(q, log q, has)``; entries that do not count have q = 0."""
-    t = torch.where((ids >= 0) & (ids < vocab), t, -math.inf) / temperature
+    entry = (ids >= 0) & (ids < vocab) & (t != -math.inf)
     if t.shape[-1] == 0:
         return t, t, torch.zeros(t.shape[0], dtype=torch.bool, device=t.device)
-    has = t.amax(-1) != -math.inf
+    has = entry.any(-1)
+    t = torch.where(entry, t, -math.inf) / temperature
     logq = torch.log_softmax(torch.where(has.unsqueeze(-1), t, 0.0), dim=-1)
-    return torch.where(has.unsqueeze(-1), logq.exp(), 0.0), logq, has
+    return torch.where(entry, logq.exp(), 0.0), logq, has
 
 
 def _statement(logits, ids, t, temperature: float, vocab_start: int, group):

@@ -123,6 +123,16 @@ def test_rows_that_do_not_count_may_hold_anything():
     assert x.grad[0].eq(0).all() and x.grad[2].eq(0).all() and x.grad.isfinite().all()
 
 
+def test_a_teacher_that_is_not_a_number_shows_in_its_token_alone():
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(3, 9, 3)
+    teacher[1, 0], teacher[1, 2], ids[1] = math.nan, -INF, torch.tensor([4, 5, 0])
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    assert loss[1].isnan() and loss[[0, 2]].isfinite().all() and grad[[0, 2]].isfinite().all()
+    assert grad[1, 4].isnan() and grad[1, 5].isnan() and grad[1, 0].isfinite()
+
+
 def test_zero_entries_and_zero_tokens():
     from steptronoss_b200.ops import fused_linear_topk_distillation, topk_distillation_loss_and_grad
 
@@ -374,6 +384,20 @@ def test_masks_repeated_and_foreign_ids_on_the_gpu(dtype):
     assert loss[8].isnan() and grad[8].isnan().all()
     rest = [0, 1, 3, 4, 6, 7]
     assert loss[rest].isfinite().all() and grad[rest].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_a_teacher_that_is_not_a_number_on_the_gpu():
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    logits, ids, teacher, w = make(3, 900, 3, device="cuda")
+    teacher[1, 0], teacher[1, 2], ids[1] = math.nan, -INF, torch.tensor([4, 5, 0], device="cuda")
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    x = logits.clone().requires_grad_()
+    tok = topk_distillation(x, ids, teacher)
+    for l, g in ((loss, grad), (tok.detach(), torch.autograd.grad(tok, x, w)[0])):
+        assert l[1].isnan() and l[[0, 2]].isfinite().all() and g[[0, 2]].isfinite().all()
+        assert g[1, 4].isnan() and g[1, 5].isnan() and g[1, 0].isfinite() and g[1, 6:].isfinite().all()
 
 
 @pytest.mark.gpu
