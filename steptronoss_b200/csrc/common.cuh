@@ -107,6 +107,14 @@ __device__ __forceinline__ bool mbar_wait_budget(uint64_t* bar, uint32_t parity,
   }
 }
 
+// ----------------------------------------------------------------------------- programmatic launches
+// A kernel launched with `overlap_launch` may start while the kernel before it in the stream still runs: it sets itself
+// up, and waits here before it touches memory that the other may write or read.  Without that attribute this returns at
+// once.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The next kernel of the stream may start setting itself up (its own wait still covers all of this kernel's writes).
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ----------------------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* d) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(d)) : "memory");
@@ -324,4 +332,10 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t d0
 int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t pitch1,
                       uint64_t pitch2, uint32_t box0, uint32_t box1, uint32_t box2, int swizzle128);
 int sm_count();
+inline cudaLaunchAttribute overlap_launch() {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
 }  // namespace stb

@@ -218,6 +218,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   cluster_sync_all();                        // the other CTA's barriers are initialised, too
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  wait_for_previous_kernel();
+  let_next_kernel_start();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -419,6 +421,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
+    wait_for_previous_kernel();
     for (int i = 0; i < min(kStages, k_blocks); ++i) load(i);     // on their way while the rest is set up
   }
   if (warp == 1) {
@@ -429,6 +432,8 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  wait_for_previous_kernel();
+  let_next_kernel_start();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -556,12 +561,12 @@ static int launch_pair(const void* xq, const void* wq, Int8GemmParams p, long lo
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2] = {overlap_launch()};
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return -static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<TY>, tw, tx, ty, p));
 }
 
@@ -580,12 +585,12 @@ static int launch_split(const void* xq, const void* wq, const Int8GemmParams& p,
   cfg.blockDim = dim3(kI8Threads);
   cfg.dynamicSmemBytes = Int8SplitSmem<BM>::kTotal;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = S;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2] = {overlap_launch()};
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = S;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = S > 1 ? 1 : 0;
+  cfg.numAttrs = S > 1 ? 2 : 1;
   return -static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_split_kernel<BM, S, TY>, tw, tx, p));
 }
 

@@ -192,6 +192,8 @@ norm_quant_kernel(const NormQuantParams p) {
   const __nv_bfloat16* xr = p.x + row * p.ldx;
   const __nv_bfloat16* dr = p.delta != nullptr ? p.delta + row * p.ldd : nullptr;
 
+  wait_for_previous_kernel();
+  let_next_kernel_start();
   uint4 v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -318,11 +320,16 @@ template <int TPR, bool E4M3, Access A>
 static cudaError_t launch_norm_quant(const NormQuantParams& p, int nv, cudaStream_t stream) {
   const int threads = TPR == 32 ? 128 : TPR;
   const long long blocks = TPR == 32 ? (p.rows + 3) / 4 : p.rows;
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (nv <= 1) norm_quant_kernel<TPR, 1, E4M3, A><<<grid, threads, 0, stream>>>(p);
-  else if (nv <= 2) norm_quant_kernel<TPR, 2, E4M3, A><<<grid, threads, 0, stream>>>(p);
-  else norm_quant_kernel<TPR, 4, E4M3, A><<<grid, threads, 0, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = overlap_launch();
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (nv <= 1) return cudaLaunchKernelEx(&cfg, norm_quant_kernel<TPR, 1, E4M3, A>, p);
+  if (nv <= 2) return cudaLaunchKernelEx(&cfg, norm_quant_kernel<TPR, 2, E4M3, A>, p);
+  return cudaLaunchKernelEx(&cfg, norm_quant_kernel<TPR, 4, E4M3, A>, p);
 }
 
 template <bool E4M3, Access A>

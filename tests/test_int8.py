@@ -238,6 +238,50 @@ def test_products_on_two_streams_and_in_a_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 40, 700])
+def test_kernels_that_follow_each_other_wait_for_their_operands(M):
+    """Each kernel may be set up while the one before it runs; tokens, weights and results are made and used in a row, the
+    same memory again and again."""
+    from steptronoss_b200 import ops
+
+    torch.manual_seed(5)
+    N, K, rounds = 3000, 1536, 12
+    xs = [torch.randn(M, K, device="cuda").to(torch.bfloat16) for _ in range(rounds)]
+    ws = [torch.randn(N, K, device="cuda").to(torch.bfloat16) for _ in range(rounds)]
+    gain = torch.ones(K, dtype=torch.bfloat16, device="cuda")
+
+    def one(x, w):
+        wq, sw = ops.quantize_rows_int8(w)
+        s, q, sq = ops.add_rmsnorm_quant(x, x, gain)
+        y = ops.gemm_int8(q, sq, wq, sw)
+        y2 = ops.linear_int8(y[:, :K], wq, sw)
+        return s, y, y2
+
+    want = []
+    for x, w in zip(xs, ws):
+        torch.cuda.synchronize()
+        wq, sw = ops.quantize_rows_int8(w)
+        torch.cuda.synchronize()
+        s, q, sq = ops.add_rmsnorm_quant(x, x, gain)
+        torch.cuda.synchronize()
+        y = ops.gemm_int8(q, sq, wq, sw)
+        torch.cuda.synchronize()
+        q2, s2 = ops.quantize_rows_int8(y[:, :K])
+        torch.cuda.synchronize()
+        want.append((s, y, ops.gemm_int8(q2, s2, wq, sw)))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = [one(x, w) for x, w in zip(xs, ws)]
+        assert all(torch.equal(a, b) for g, t in zip(got, want) for a, b in zip(g, t))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [one(x, w) for x, w in zip(xs, ws)]
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(a, b) for g, t in zip(got, want) for a, b in zip(g, t))
+
+
+@pytest.mark.gpu
 def test_gpu_refusals():
     from steptronoss_b200 import ops
 
