@@ -379,7 +379,8 @@ struct Int8SplitSmem {
 // of that column into that CTA's shared memory (over the operand ring, which nobody reads any more), and after one more
 // cluster barrier each CTA adds, scales and writes its columns.
 //
-// Bound: the weights' bytes.  Two CTAs fit on an SM, so up to 296 stream at a time and none waits for a second wave.
+// Bound: the weights' bytes.  Two CTAs fit on an SM, so up to 296 stream at a time (48 x 24576 x 4096, 192 tiles: 33 us with
+// one CTA per SM in two waves, 23 us).
 template <int BM, int S, typename TY>
 __global__ void __launch_bounds__(kI8Threads, 2)
 gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,

@@ -629,6 +629,28 @@ def test_fused_head_adds_into_main_grad():
 
 
 @pytest.mark.gpu
+def test_gradient_agrees_with_differences_on_the_gpu():
+    from steptronoss_b200.ops import topk_distillation
+
+    T, V, K, tau, h = 5, 400, 7, 1.5, 0.02
+    logits, ids, teacher, w = make(T, V, K, seed=12, device="cuda")
+    ids[0, 1] = ids[0, 0]
+    d = torch.randint(0, 2, (T, V), device="cuda").float() * 2 - 1
+    x = logits.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(topk_distillation(x, ids, teacher, tau), x, torch.ones(T, device="cuda"))
+    slope = (topk_distillation(logits + h * d, ids, teacher, tau) - topk_distillation(logits - h * d, ids, teacher, tau)) / (2 * h)
+    _, wgrad, p, q = oracle(logits, ids, teacher, tau)
+    loss_tol, _ = bounds(logits.cpu(), teacher.cpu(), tau, p, q, wgrad, torch.ones(T, dtype=torch.float64), torch.float32)
+    # the loss is off by loss_tol on either side; along d = +-1 its third derivative is a third central moment of values in
+    # [-1, 1] over tau^3, at most 2 / tau^3; logits +- h d are rounded by 2^-24 of 15 at most, times a gradient of size 1
+    tol = loss_tol / h + h * h / 6 * 2 / tau ** 3 + 15 * 2.0 ** -24 / h + 1e-5
+    assert ((grad * d).sum(1).double() - slope.double()).abs().max() <= tol
+    # and that says something: logits of spread 30 at most give A <= 1.4427 * 30 / 1.5 + 20 = 49, so that loss_tol / h is at
+    # most (4 * 49 + 212 + 2 * 49 * (2 * 49 + 48)) 2^-24 / 0.02 = 0.044, the other terms 2e-4; the slopes are about 0.4
+    assert tol < 0.05
+
+
+@pytest.mark.gpu
 def test_kernels_on_a_side_stream_and_in_a_graph():
     from steptronoss_b200.ops import topk_distillation_loss_and_grad
 

@@ -282,6 +282,44 @@ def test_kernels_that_follow_each_other_wait_for_their_operands(M):
 
 
 @pytest.mark.gpu
+def test_kernels_behind_a_fork_and_a_join_of_streams():
+    """A product directly behind an event that another stream recorded, eagerly and in a captured graph."""
+    from steptronoss_b200 import ops
+
+    xq, sx, wq, sw = operands(33, 4096, 2048, "cuda", seed=7)
+    x = torch.randn(33, 2048, device="cuda").to(torch.bfloat16)
+    side = torch.cuda.Stream()
+    big = torch.randn(4096, 4096, device="cuda")
+
+    def work():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            slow = big @ big                                     # keeps the side stream busy before it quantises
+            q, s = ops.quantize_rows_int8(x + (slow[:33, :2048] * 0).to(torch.bfloat16))
+        first = ops.gemm_int8(xq, sx, wq, sw)
+        main.wait_stream(side)
+        second = ops.gemm_int8(q, s, wq, sw)                     # right behind the join
+        for t in (slow, q, s):
+            t.record_stream(main)
+        return first, second
+
+    want = ops.gemm_int8(xq, sx, wq, sw), ops.linear_int8(x, wq, sw)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(work(), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_gpu_refusals():
     from steptronoss_b200 import ops
 
