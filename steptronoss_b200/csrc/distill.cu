@@ -37,6 +37,7 @@ struct DistillParams {
   const float* weight;          // [T] or nullptr (1)
   float* loss;                  // [T] or nullptr
   float4* stats;                // [T] or nullptr
+  const float4* given;          // row kernel: finished statistics, only the gradient is wanted
   float* picked;                // stats kernel: [T][K] student logit at each id, 0 where it is not in this shard
   long long ld, ldg, ld_ids, ld_t;
   long long vocab_start, vocab_total;
@@ -286,6 +287,9 @@ __device__ __forceinline__ void block_merge(float& m, float& s, float2* red) {
 //
 // Loads, entries and the cluster's exchange thus run beside the arithmetic; nothing waits for the whole CTA.
 //
+// Without a gradient there is no pass 2, with given statistics no pass 1 and no exchange: a chunk is then released as soon
+// as it has been read, a row needs no room, and with enough rows one CTA takes a whole one.
+//
 // Bound: DRAM for fp32 logits (2048 x 151936: 397 us, 6.27 TB/s of 6.55 measured).  For bf16 the exponentials (two per
 // element, 16 a cycle and SM: 277 us of 4096 x 151936) and the issue slots (15 per element, half of them for what a row costs
 // a warp whatever its length) are both busy for about 60 % of the time: 471 us, 5.3 TB/s.  Measured around this point, same
@@ -301,7 +305,7 @@ constexpr int kMaxChunks = 12;
 struct RowPlan {
   int per;             // granules per CTA
   int chunks;          // per slice
-  int ring;            // chunks in shared memory, at least those of a slice
+  int ring;            // chunks in shared memory, at least those of a slice where both passes are made
   int kpad;            // K rounded up to 4
 };
 struct RowBars {
@@ -511,7 +515,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
     failed = 0;
     fence_barrier_init();
   }
-  {
+  if (p.grad != nullptr) {
     uint32_t* bitmaps = reinterpret_cast<uint32_t*>(entry_base + 2 * entry_bytes(plan.kpad));
     for (int i = threadIdx.x; i < 2 * bitmap_bytes(plan.per, n) / 4; i += kRowThreads) bitmaps[i] = 0;
   }
@@ -521,9 +525,10 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
     cluster_wait();
   }
 
-  // The rows of this cluster: number 0 is its own; number i > 0 is requested after the exchange of row i - 2, when every
-  // warp of every CTA has read the answers up to i - 2, of which four are kept: number i in place (i - 1) % 4, the
-  // (i - 1) / 4-th answer there.  No request follows a refused one.
+  // The rows of this cluster: number 0 is its own; number i > 0 is requested after the exchange of row i - 2 (with given
+  // statistics, and one CTA: when the entries of that row are prepared, which follows the end of row i - 4), when every
+  // warp of every CTA has read the answers up to i - 4 at least, of which four are kept: number i in place (i - 1) % 4,
+  // the (i - 1) / 4-th answer there.  No request follows a refused one.
   auto request = [&](int i) {              // by one thread of each CTA
     const int at = (i - 1) & 3;
     mbar_arrive_expect_tx(&bars.claim[at], 16);
@@ -588,6 +593,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
       const Granules<T> gr(src, p.V);
       const int e0 = rank * plan.per * n - gr.lead, e1 = e0 + plan.per * n;
       const float w = p.weight != nullptr ? p.weight[row] : 1.f;
+      const float4 given = p.given != nullptr ? p.given[row] : make_float4(0.f, 0.f, 0.f, 0.f);
       float tmax = -INFINITY;
       bool bad = false;                    // fmaxf drops a NaN; it has to reach the loss
       int own = 0;
@@ -629,24 +635,37 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
       if (__any_sync(0xffffffffu, bad)) tmax = __uint_as_float(0x7FC00000u);
       const bool some = tmax != -INFINITY;
       float tsum = 0.f;
-      for (int j = lane; j < p.K; j += 32) {
-        const float e = some ? ex2((elq[j] - tmax) * c) : 0.f;
-        eq[j] = e;
-        tsum += e;
+      if (p.given != nullptr) {
+        tmax = given.z;
+        tsum = given.w;
+      } else {
+        for (int j = lane; j < p.K; j += 32) {
+          const float e = some ? ex2((elq[j] - tmax) * c) : 0.f;
+          eq[j] = e;
+          tsum += e;
+        }
+        tsum = warp_total(tsum);
       }
-      tsum = warp_total(tsum);
       // what the compute warps need, and the word that the logits at the entries have been read
       if (lane == 0) {
         hd.tmax = tmax;
         hd.tsum = tsum;
         hd.weight = w;
+        if (p.given != nullptr) {
+          hd.top = given.x;
+          hd.sum = given.y;
+        }
       }
       mbar_arrive_warp(&bars.e_full[b]);
-      const float inv = some ? __fdiv_rn(1.f, tsum) : 0.f, log_tsum = some ? log2f(tsum) : 0.f;
-      for (int j = lane; j < p.K; j += 32) {
-        eq[j] *= inv;
-        elq[j] = (elq[j] - tmax) * c - log_tsum;
+      const float inv = some ? __fdiv_rn(1.f, tsum) : 0.f;
+      if (p.loss != nullptr) {
+        const float log_tsum = some ? log2f(tsum) : 0.f;
+        for (int j = lane; j < p.K; j += 32) {
+          eq[j] *= inv;
+          elq[j] = (elq[j] - tmax) * c - log_tsum;
+        }
       }
+      if (p.grad == nullptr) own = 0;
       // the same id twice?  One bit per element of the slice tells, and only then are the equal ids looked for
       bool twice = false;
       for (int j = lane; j < own; j += 32) {
@@ -718,6 +737,10 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
       // pass 1: a thread that has seen nothing but -inf adds exp2(-inf) = 0
       float top = -INFINITY;
       uint64_t acc[2] = {0, 0};                       // two pairs of sums
+      auto leave = [&] {                              // by the whole warp, when a wait has run out
+        report_error(p.status, kErrEpilogueWait);
+        failed = 1;
+      };
       auto raise = [&](float m) {
         if (m > top) {
           const float scale = ex2(top - m);
@@ -738,57 +761,64 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           for (int j = 0; j < kP; ++j) acc[j & 1] = add2(acc[j & 1], ex2_2(fma2(f[j], c2, minus)));
         }
       };
-      for (int k = 0; k < plan.chunks; ++k) {
-        const int k0 = sl.g0 + k * kChunk;
-        ok = __all_sync(0xffffffffu, mbar_wait_soon(&bars.full[slot1], lap));
-        if (!ok) break;
-        const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot1 * kChunk;
-        const int lo = sl.gs - k0, hi = min(sl.ge - k0, kChunk);
-        const int g = threadIdx.x;
-        uint4 v[kU];
-        if (lo <= 0 && hi == kChunk) {
+      float sum = 0.f;
+      if (p.given != nullptr) {
+        ok = __all_sync(0xffffffffu, mbar_wait_soon(&bars.e_full[b], phase));
+        if (!ok) { leave(); break; }
+        top = head[b].top;
+        sum = head[b].sum;
+      } else {
+        for (int k = 0; k < plan.chunks; ++k) {
+          const int k0 = sl.g0 + k * kChunk;
+          ok = __all_sync(0xffffffffu, mbar_wait_soon(&bars.full[slot1], lap));
+          if (!ok) break;
+          const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot1 * kChunk;
+          const int lo = sl.gs - k0, hi = min(sl.ge - k0, kChunk);
+          const int g = threadIdx.x;
+          uint4 v[kU];
+          if (lo <= 0 && hi == kChunk) {
 #pragma unroll
-          for (int u = 0; u < kU; ++u) v[u] = chunk[g + u * kRowCompute];
-          take(v);
-        } else if (g < hi) {
+            for (int u = 0; u < kU; ++u) v[u] = chunk[g + u * kRowCompute];
+            take(v);
+          } else if (g < hi) {
 #pragma unroll
-          for (int u = 0; u < kU; ++u) {
-            const int i = g + u * kRowCompute;
-            v[u] = i >= lo && i < hi ? chunk[i] : make_uint4(kNone, kNone, kNone, kNone);
+            for (int u = 0; u < kU; ++u) {
+              const int i = g + u * kRowCompute;
+              v[u] = i >= lo && i < hi ? chunk[i] : make_uint4(kNone, kNone, kNone, kNone);
+            }
+            take(v);
           }
-          take(v);
+          if (p.grad == nullptr) mbar_arrive_warp(&bars.empty[slot1]);
+          if (++slot1 == plan.ring) { slot1 = 0; lap ^= 1; }
         }
-        if (p.grad == nullptr) mbar_arrive_warp(&bars.empty[slot1]);
-        if (++slot1 == plan.ring) { slot1 = 0; lap ^= 1; }
-      }
-      if (edge >= 0) {
-        const float base = raise(x_edge * c);
-        acc[0] = add2(acc[0], pair(ex2(fmaf(x_edge, c, base)), 0.f));
-      }
-      float sum, sum1;
-      unpair(add2(acc[0], acc[1]), sum, sum1);
-      sum += sum1;
-      warp_merge(top, sum);
-      // the logits at the entries have been read: only now may another CTA overwrite them
-      ok = ok && mbar_wait_soon(&bars.e_full[b], phase);
-      if (threadIdx.x == 0) mbar_arrive_expect_tx(&bars.xchg[b], C * kRowWarps * 8);
-      __syncwarp();
-      if (lane < C) send_pair(&part[b][rank * kRowWarps + warp], &bars.xchg[b], lane, top, sum);
-      ok = ok && mbar_wait_soon(&bars.xchg[b], phase);
-      if (!__all_sync(0xffffffffu, ok)) {
-        report_error(p.status, kErrEpilogueWait);
-        failed = 1;
-        break;
-      }
-      constexpr int kPairs = C * kRowWarps;
-      top = lane < kPairs ? part[b][lane].x : -INFINITY;
-      sum = lane < kPairs ? part[b][lane].y : 0.f;
+        if (edge >= 0) {
+          const float base = raise(x_edge * c);
+          acc[0] = add2(acc[0], pair(ex2(fmaf(x_edge, c, base)), 0.f));
+        }
+        float sum1;
+        unpair(add2(acc[0], acc[1]), sum, sum1);
+        sum += sum1;
+        warp_merge(top, sum);
+        // the logits at the entries have been read: only now may another CTA overwrite them
+        ok = ok && mbar_wait_soon(&bars.e_full[b], phase);
+        if (threadIdx.x == 0) mbar_arrive_expect_tx(&bars.xchg[b], C * kRowWarps * 8);
+        __syncwarp();
+        if (lane < C) send_pair(&part[b][rank * kRowWarps + warp], &bars.xchg[b], lane, top, sum);
+        ok = ok && mbar_wait_soon(&bars.xchg[b], phase);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) { leave(); break; }
+        constexpr int kPairs = C * kRowWarps;
+        top = lane < kPairs ? part[b][lane].x : -INFINITY;
+        sum = lane < kPairs ? part[b][lane].y : 0.f;
 #pragma unroll
-      for (int i = 32; i < kPairs; i += 32) merge(top, sum, part[b][lane + i].x, part[b][lane + i].y);
-      warp_merge(top, sum);
+        for (int i = 32; i < kPairs; i += 32) merge(top, sum, part[b][lane + i].x, part[b][lane + i].y);
+        warp_merge(top, sum);
+      }
       if (threadIdx.x == 0) {
-        head[b].top = top;
-        head[b].sum = sum;
+        if (p.given == nullptr) {
+          head[b].top = top;
+          head[b].sum = sum;
+        }
         if (answered(it + 1) && granted(it + 1) >= 0) request(it + 2);
       }
       if (p.grad != nullptr) {
@@ -814,6 +844,10 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         };
         for (int k = 0; k < plan.chunks; ++k) {
           const int k0 = sl.g0 + k * kChunk;
+          if (p.given != nullptr) {                   // otherwise pass 1 has waited for it
+            ok = __all_sync(0xffffffffu, mbar_wait_soon(&bars.full[slot2], lap));
+            if (!ok) break;
+          }
           const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot2 * kChunk;
           const int lo = sl.gs - k0, hi = min(sl.ge - k0, kChunk);
           const int g = threadIdx.x;
@@ -832,8 +866,12 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
             }
           }
           mbar_arrive_warp(&bars.empty[slot2]);
-          if (++slot2 == plan.ring) slot2 = 0;
+          if (++slot2 == plan.ring) {
+            slot2 = 0;
+            if (p.given != nullptr) lap ^= 1;
+          }
         }
+        if (!ok) { leave(); break; }
         if (edge >= 0) Lane<TO>::store(dst + edge, zero ? 0.f : ex2(fmaf(x_edge, c, -top)) * scale);
       }
       mbar_arrive_warp(&bars.e_empty[b]);
@@ -1021,14 +1059,16 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   plan.per = static_cast<int>((max_granules(p.V, n) + C - 1) / C);
   plan.chunks = (plan.per + kChunk - 1) / kChunk;
   plan.kpad = (p.K + 3) & ~3;
-  const int side = 2 * (entry_bytes(plan.kpad) + bitmap_bytes(plan.per, n));
-  // two CTAs per SM where a slice fits into half of it, so that one computes while the other waits; else one CTA
+  const int side = 2 * (entry_bytes(plan.kpad) + (p.grad != nullptr ? bitmap_bytes(plan.per, n) : 0));
+  // two CTAs per SM where a slice (or two chunks of a row that is only passed through) fits into half of it, so that one
+  // computes while the other waits; else one CTA
+  const int need = p.grad != nullptr && p.given == nullptr ? plan.chunks : 2;
   for (int ctas = 2; ctas >= 1; --ctas) {
     plan.ring = (kRowSmem / ctas - 2048 - side) / (kChunk * 16);
-    if (plan.ring >= plan.chunks) break;
+    if (plan.ring >= need) break;
   }
   if (plan.ring > kMaxChunks) plan.ring = kMaxChunks;
-  if (plan.ring < plan.chunks) return cudaErrorInvalidValue;
+  if (plan.ring < need) return cudaErrorInvalidValue;
   const int smem = plan.ring * kChunk * 16 + side;
   auto kernel = distill_row_kernel<T, TO, C>;
   int dev = 0;
@@ -1060,8 +1100,12 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
 // merging and exchanging) 687 us.
 constexpr int kHalfSlice = 88 * 1024;
 
+// Whether there are rows enough for one CTA each where a row is only passed through.
+static bool many_rows(int T) { return T >= 2 * sm_count(); }
+
 template <typename T, typename TO>
 static cudaError_t run_row(const DistillParams& p, cudaStream_t stream) {
+  if ((p.grad == nullptr && many_rows(p.T)) || p.given != nullptr) return launch_row<T, TO, 1>(p, stream);
   const long long bytes = max_granules(p.V, Lane<T>::n) * 16;
   int c = 1;
   while (c < 8 && bytes > static_cast<long long>(c) * kHalfSlice) c *= 2;
@@ -1146,13 +1190,23 @@ extern "C" int stb_distill_loss(const void* ids, int ids64, long long ld_ids, co
 extern "C" int stb_distill_grad(const void* logits, long long ld, void* grad, long long ldg, const void* ids, int ids64,
                                 long long ld_ids, const float* teacher, long long ld_t, const float* weight,
                                 const float* stats, int T, int V, int K, long long vocab_start, long long vocab_total,
-                                float inv_tau, int elem_bytes, int grad_bytes, cudaStream_t stream) {
+                                float inv_tau, int elem_bytes, int grad_bytes, int* status, cudaStream_t stream) {
   if (T == 0) return 0;
   DistillParams p{};
   p.logits = logits; p.ld = ld; p.grad = grad; p.ldg = ldg; p.ids = ids; p.ids64 = ids64; p.ld_ids = ld_ids;
   p.teacher = teacher; p.ld_t = ld_t; p.weight = weight; p.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
   p.T = T; p.V = V; p.K = K; p.vocab_start = vocab_start; p.vocab_total = vocab_total; p.inv_tau = inv_tau;
   if (!distill_args_ok(p) || grad == nullptr || !distill_types_ok(elem_bytes, grad_bytes)) return -kErrBadArgument;
+  if (logits != grad && vocab_start == 0 && vocab_total == V && V <= stb_distill_row_limit(elem_bytes) && many_rows(T)) {
+    p.given = p.stats;
+    p.stats = nullptr;
+    p.status = status;
+    cudaError_t e;
+    if (elem_bytes == 2) e = run_row<__nv_bfloat16, __nv_bfloat16>(p, stream);
+    else if (grad_bytes == 4) e = run_row<float, float>(p, stream);
+    else e = run_row<float, __nv_bfloat16>(p, stream);
+    return -static_cast<int>(e);
+  }
   const int n = 16 / elem_bytes;
   const long long chunks = (max_granules(V, n) + kDsThreads * kGradVec - 1) / (kDsThreads * kGradVec);
   if (chunks * T > 0x7FFFFFFFll) return -kErrBadArgument;

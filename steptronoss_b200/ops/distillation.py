@@ -36,7 +36,7 @@ native.register_signature("stb_distill_stats", [P, L, P, I, L, P, L, P, P, I, I,
 native.register_signature("stb_distill_loss", [P, I, L, P, L, P, P, P, I, I, L, F, P])
 native.register_signature("stb_distill_total", [P, P, I, P, P])
 native.register_signature("stb_distill_scale", [P, P, P, L, P])
-native.register_signature("stb_distill_grad", [P, L, P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, I, P])
+native.register_signature("stb_distill_grad", [P, L, P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, I, P, P])
 
 
 # --------------------------------------------------------------------------------------------------- arguments
@@ -197,11 +197,12 @@ def _join_shards(stats, picked, group) -> None:
 
 def _grad_kernel(x, ids, t, temperature, weights, stats, grad, vocab_start=0, vocab=None):
     T, V = x.shape
+    index = x.get_device()
     rc = native.launch(
-        native.load().stb_distill_grad, x.get_device(), x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0),
+        native.load().stb_distill_grad, index, x.data_ptr(), x.stride(0), grad.data_ptr(), grad.stride(0),
         ids.data_ptr(), int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0), weights.data_ptr(),
         stats.data_ptr(), T, V, ids.shape[1], vocab_start, V if vocab is None else vocab, 1.0 / temperature,
-        x.element_size(), grad.element_size())
+        x.element_size(), grad.element_size(), native.status_ptr(index))
     if rc:
         native.check(rc, f"distill_grad T={T} V={V} K={ids.shape[1]}")
     count_launch()
