@@ -7,8 +7,9 @@
 // and a zero gradient whatever its logits hold, and so has a row of weight 0.  The same id may come several times.
 //
 // Three kernels:
-//   distill_row_kernel    the row stays in the shared memory of a thread-block cluster: one read of the logits gives the
-//                         loss, the statistics and (optionally) the gradient, which may overwrite the logits
+//   distill_row_kernel    a row on a thread-block cluster, its logits in shared memory as far as they fit and for the
+//                         rest once more from L2: one read of the logits from DRAM gives the loss, the statistics and
+//                         (optionally) the gradient, which may overwrite the logits
 //   distill_stats_kernel  a row of any length, or the local part of a vocabulary that is sharded over ranks:
 //                         max, sum of exponentials and the student's logits at the teacher's ids
 //   distill_grad_kernel   the gradient from finished statistics (backward pass; sharded or very long rows)
@@ -274,27 +275,30 @@ __device__ __forceinline__ void block_merge(float& m, float& s, float2* red) {
 // ------------------------------------------------------------------------------------------- whole rows, one pass
 // One cluster of C CTAs is launched per row; a running cluster takes over the rows of clusters that have not started
 // (clusterlaunchcontrol), so that its set-up is paid once and a cluster on less busy SMs does more rows (with fixed rows
-// the first clusters were done after 385 us of 495).  Each CTA has a contiguous slice of the row's granules, which stays
-// in shared memory between the two passes over it:
+// the first clusters were done after 385 us of 495).  Each CTA has a contiguous slice of the row's granules and makes two
+// passes over it:
 //
-//   producer warp   bulk copies of 16 KB chunks into a ring that runs on from row to row: a chunk that pass 2 has read is
-//                   filled with the next row's logits at once
+//   producer warp   bulk copies of 16 KB chunks into a ring that runs on from row to row.  The last chunks of a slice, as
+//                   many as the ring holds, stay there for pass 2, which begins with them; the others are loaded again,
+//                   from L2, where the first load asked for them to be kept
 //   entries warps   two, for even and odd rows: the teacher's entries of a coming row, their statistics and the list of
 //                   those that fall into this CTA's slice; behind pass 2 the loss and the gradient at the entries
 //   compute warps   pass 1: (top, sum) of the slice.  Every warp sends its pair to all CTAs of the cluster (st.async onto
-//                   their mbarriers) and merges all pairs when they are there.  Pass 2: the gradient from the same shared
-//                   memory, straight to global memory
+//                   their mbarriers) and merges all pairs when they are there.  Pass 2: the gradient, straight to global
+//                   memory
 //
 // Loads, entries and the cluster's exchange thus run beside the arithmetic; nothing waits for the whole CTA.
 //
 // Without a gradient there is no pass 2, with given statistics no pass 1 and no exchange: a chunk is then released as soon
-// as it has been read, a row needs no room, and with enough rows one CTA takes a whole one.
+// as it has been read, and with enough rows one CTA takes a whole one (4096 x 151936 bf16: 198 us and 399 us, 6.3 and 6.2
+// TB/s of 6.55 measured).
 //
-// Bound: DRAM for fp32 logits (2048 x 151936: 397 us, 6.27 TB/s of 6.55 measured).  For bf16 the exponentials (two per
-// element, 16 a cycle and SM: 277 us of 4096 x 151936) and the issue slots (15 per element, half of them for what a row costs
-// a warp whatever its length) are both busy for about 60 % of the time: 471 us, 5.3 TB/s.  Measured around this point, same
-// size: 4, 6 or 12 compute warps 554, 588, 480 us; 3 or 4 smaller CTAs on an SM 513-570; two or eight granules per thread and
-// chunk 553, 580; every fourth exponential by a polynomial instead of the special-function unit 522 against 524 at the time.
+// Bound: DRAM for fp32 logits (2048 x 151936: 390 us, 6.4 TB/s).  For bf16 the exponentials (two per element, 16 a cycle
+// and SM: 277 us of 4096 x 151936) and the issue slots are busy for 60 % of the time beside it: 457 us, 5.5 TB/s.  What a row
+// costs a warp whatever its length (set-up, merging, exchange: half of the instructions with slices of 76 KB) asks for
+// long slices; measured, same size, 1, 2, 4, 8 CTAs per row: 468, 457, 488, 699 us (fp32: 551, 456, 391, 409).  Loading
+// nothing again (slices of 76 KB, all kept): 488.  4, 6, 10, 12 compute warps (at their best slice): 554, 588, 476, 458.
+// Every fourth exponential by a polynomial instead of the special-function unit: 522 against 524 at the time.
 constexpr int kU = 4;                            // granules per compute thread and chunk
 constexpr int kRowWarps = 8;                     // compute warps
 constexpr int kRowCompute = 32 * kRowWarps;
@@ -306,6 +310,7 @@ struct RowPlan {
   int per;             // granules per CTA
   int chunks;          // per slice
   int ring;            // chunks in shared memory, at least those of a slice where both passes are made
+  int keep;            // last chunks of a slice that stay in the ring between the two passes; the others are loaded again
   int kpad;            // K rounded up to 4
 };
 struct RowBars {
@@ -332,9 +337,18 @@ __device__ __forceinline__ void send_pair(float2* slot, uint64_t* bar, uint32_t 
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
                ::"r"(dst), "f"(a), "f"(b), "r"(rbar) : "memory");
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+// `how`: 0 as usual, 1 keep in L2 (it is read again soon), 2 drop from L2 (it was the last time)
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, int how) {
+  if (how == 0) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+    return;
+  }
+  uint64_t policy;
+  if (how == 1) asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
+  else asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy) : "memory");
 }
 // Two fp32 at once: one instruction on this architecture.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
@@ -408,12 +422,12 @@ __device__ __forceinline__ void store_pairs(TO* at, bool aligned, const uint64_t
   for (int j = 0; j < NP; ++j) unpair(f[j], v[2 * j], v[2 * j + 1]);
   if (aligned) {
     if constexpr (sizeof(TO) == 4) {
-      *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+      __stcs(reinterpret_cast<float4*>(at), make_float4(v[0], v[1], v[2], v[3]));
     } else if constexpr (NP == 4) {
-      *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
-                                                 pack_bf16(v[6], v[7]));
+      __stcs(reinterpret_cast<uint4*>(at), make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                                                 pack_bf16(v[6], v[7])));
     } else {
-      *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+      __stcs(reinterpret_cast<uint2*>(at), make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])));
     }
   } else {
 #pragma unroll
@@ -500,6 +514,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
   const int first_row = blockIdx.x / C;
   uint8_t* entry_base = dyn + plan.ring * kChunk * 16;
   const float c = p.inv_tau * kLog2e;
+  const bool both = p.grad != nullptr && p.given == nullptr;       // passes
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < plan.ring; ++i) {
@@ -555,11 +570,13 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
     uint32_t lap = 0;                      // parity of the ring's passes
     bool ok = true, more = true;
     long long row = first_row;
-    for (int i = 1; ok && more; more = ok && next_row(i++, row)) {
+    for (int number = 1; ok && more; more = ok && next_row(number++, row)) {
       const T* src = static_cast<const T*>(p.logits) + row * p.ld;
       const Granules<T> gr(src, p.V);
       const Slice<T> sl(gr, rank, plan.per, p.V);
-      for (int k = 0; k < plan.chunks; ++k) {
+      const int again = both ? plan.chunks - plan.keep : 0;
+      for (int i = 0; i < plan.chunks + again; ++i) {
+        const int k = i < plan.chunks ? i : i - plan.chunks;
         ok = __all_sync(0xffffffffu, !failed && mbar_wait_idle(&bars.empty[slot], lap ^ 1, 100));
         if (!ok) { report_error(p.status, kErrProducerWait); failed = 1; break; }
         if (lane == 0) {
@@ -568,7 +585,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
             const uint32_t bytes = static_cast<uint32_t>(b - a) * 16;
             mbar_arrive_expect_tx(&bars.full[slot], bytes);
             bulk_load(dyn + (slot * kChunk + a - k0) * 16, src + (static_cast<long long>(a) * n - gr.lead), bytes,
-                      &bars.full[slot]);
+                      &bars.full[slot], i < again ? 1 : again > 0 ? 2 : 0);
           } else {
             mbar_arrive(&bars.full[slot]);
           }
@@ -722,8 +739,15 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
     constexpr int kP = Pairs<T>::n;
     constexpr uint32_t kNone = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;    // -inf
     const uint64_t c2 = pair(c, c);
-    int it = 0, slot1 = 0, slot2 = 0;      // ring positions of the two passes
+    // Chunks are awaited in the order of their loads, at ring position `slot` in its `lap`-th round, and released in the
+    // same order: what stays between the passes is released by pass 2, which goes to it first, at position `slot2`.
+    const int through = both ? plan.chunks - plan.keep : plan.chunks;
+    int it = 0, slot = 0;
     uint32_t lap = 0;
+    auto arrived = [&] { return __all_sync(0xffffffffu, mbar_wait_soon(&bars.full[slot], lap)); };
+    auto advance = [&] {
+      if (++slot == plan.ring) { slot = 0; lap ^= 1; }
+    };
     long long row = first_row;
     for (bool more = true; more; more = next_row(++it, row)) {
       const int b = it & 1;
@@ -770,9 +794,9 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
       } else {
         for (int k = 0; k < plan.chunks; ++k) {
           const int k0 = sl.g0 + k * kChunk;
-          ok = __all_sync(0xffffffffu, mbar_wait_soon(&bars.full[slot1], lap));
+          ok = arrived();
           if (!ok) break;
-          const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot1 * kChunk;
+          const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot * kChunk;
           const int lo = sl.gs - k0, hi = min(sl.ge - k0, kChunk);
           const int g = threadIdx.x;
           uint4 v[kU];
@@ -788,8 +812,8 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
             }
             take(v);
           }
-          if (p.grad == nullptr) mbar_arrive_warp(&bars.empty[slot1]);
-          if (++slot1 == plan.ring) { slot1 = 0; lap ^= 1; }
+          if (k < through) mbar_arrive_warp(&bars.empty[slot]);
+          advance();
         }
         if (edge >= 0) {
           const float base = raise(x_edge * c);
@@ -811,7 +835,8 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         top = lane < kPairs ? part[b][lane].x : -INFINITY;
         sum = lane < kPairs ? part[b][lane].y : 0.f;
 #pragma unroll
-        for (int i = 32; i < kPairs; i += 32) merge(top, sum, part[b][lane + i].x, part[b][lane + i].y);
+        for (int i = 32; i < kPairs; i += 32)
+          if (lane + i < kPairs) merge(top, sum, part[b][lane + i].x, part[b][lane + i].y);
         warp_merge(top, sum);
       }
       if (threadIdx.x == 0) {
@@ -842,13 +867,9 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           for (int j = 0; j < kP; ++j) f[j] = mul2(ex2_2(fma2(f[j], c2, minus)), scale2);
           store_pairs<TO, kP>(out + granule * n, aligned, f);
         };
-        for (int k = 0; k < plan.chunks; ++k) {
+        auto finish = [&](int k, int at) {            // chunk k of the slice, at this place of the ring
           const int k0 = sl.g0 + k * kChunk;
-          if (p.given != nullptr) {                   // otherwise pass 1 has waited for it
-            ok = __all_sync(0xffffffffu, mbar_wait_soon(&bars.full[slot2], lap));
-            if (!ok) break;
-          }
-          const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + slot2 * kChunk;
+          const uint4* chunk = reinterpret_cast<const uint4*>(dyn) + at * kChunk;
           const int lo = sl.gs - k0, hi = min(sl.ge - k0, kChunk);
           const int g = threadIdx.x;
           if (zero) {
@@ -865,10 +886,20 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
               if (i >= lo && i < hi) give(chunk[i], k0 + i);
             }
           }
-          mbar_arrive_warp(&bars.empty[slot2]);
-          if (++slot2 == plan.ring) {
-            slot2 = 0;
-            if (p.given != nullptr) lap ^= 1;
+          mbar_arrive_warp(&bars.empty[at]);
+        };
+        int kept = both ? plan.keep : 0;              // chunks that pass 1 has left in the ring, then those of another load
+        int slot2 = slot - kept < 0 ? slot - kept + plan.ring : slot - kept;
+        const int from = plan.chunks - kept;
+        for (int i = 0; i < plan.chunks; ++i) {
+          if (i < kept) {
+            finish(from + i, slot2);
+            if (++slot2 == plan.ring) slot2 = 0;
+          } else {
+            ok = arrived();
+            if (!ok) break;
+            finish(i - kept, slot);
+            advance();
           }
         }
         if (!ok) { leave(); break; }
@@ -1060,15 +1091,14 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   plan.chunks = (plan.per + kChunk - 1) / kChunk;
   plan.kpad = (p.K + 3) & ~3;
   const int side = 2 * (entry_bytes(plan.kpad) + (p.grad != nullptr ? bitmap_bytes(plan.per, n) : 0));
-  // two CTAs per SM where a slice (or two chunks of a row that is only passed through) fits into half of it, so that one
-  // computes while the other waits; else one CTA
-  const int need = p.grad != nullptr && p.given == nullptr ? plan.chunks : 2;
+  // two CTAs per SM where that leaves each a ring of two chunks, so that one computes while the other waits; else one CTA
   for (int ctas = 2; ctas >= 1; --ctas) {
     plan.ring = (kRowSmem / ctas - 2048 - side) / (kChunk * 16);
-    if (plan.ring >= need) break;
+    if (plan.ring >= 2) break;
   }
   if (plan.ring > kMaxChunks) plan.ring = kMaxChunks;
-  if (plan.ring < need) return cudaErrorInvalidValue;
+  if (plan.ring < 2) return cudaErrorInvalidValue;
+  plan.keep = plan.chunks < plan.ring ? plan.chunks : plan.ring;
   const int smem = plan.ring * kChunk * 16 + side;
   auto kernel = distill_row_kernel<T, TO, C>;
   int dev = 0;
@@ -1095,10 +1125,9 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p, plan);
 }
 
-// CTAs per row: the fewest whose slice of it leaves room for two CTAs on an SM, more (up to 8) while the rows alone do not
-// fill the SMs.  Measured for 4096 rows of 151936 bf16: 4 CTAs 500 us, 8 CTAs (half the slice, the same cost per row of
-// merging and exchanging) 687 us.
-constexpr int kHalfSlice = 88 * 1024;
+// CTAs per row: the fewest whose slices are not much longer than a ring (96 KB with two CTAs per SM), so that most of a
+// slice is not loaded again, more (up to 8) while the rows alone do not fill the SMs.
+constexpr int kWidestSlice = 160 * 1024;
 
 // Whether there are rows enough for one CTA each where a row is only passed through.
 static bool many_rows(int T) { return T >= 2 * sm_count(); }
@@ -1108,7 +1137,7 @@ static cudaError_t run_row(const DistillParams& p, cudaStream_t stream) {
   if ((p.grad == nullptr && many_rows(p.T)) || p.given != nullptr) return launch_row<T, TO, 1>(p, stream);
   const long long bytes = max_granules(p.V, Lane<T>::n) * 16;
   int c = 1;
-  while (c < 8 && bytes > static_cast<long long>(c) * kHalfSlice) c *= 2;
+  while (c < 8 && bytes > static_cast<long long>(c) * kWidestSlice) c *= 2;
   while (c < 8 && static_cast<long long>(p.T) * c < sm_count() && bytes > static_cast<long long>(c) * 4096) c *= 2;
   switch (c) {
     case 1: return launch_row<T, TO, 1>(p, stream);

@@ -11,8 +11,8 @@ lies outside the vocabulary; ids may repeat.  A token without entries has loss 0
 hold, and a token of weight 0 has gradient 0.  The factor ``tau ** 2`` that some recipes put in front is left to the
 caller's weights.
 
-The CUDA path is ``csrc/distill.cu``: a row stays in the shared memory of a thread-block cluster, so that one read of the
-logits gives the loss and the gradient.  Rows longer than the cluster holds, and vocabularies that are sharded over a
+The CUDA path is ``csrc/distill.cu``: a thread-block cluster takes a row, so that one read of the logits from DRAM gives
+the loss and the gradient.  Rows longer than the cluster holds, and vocabularies that are sharded over a
 group, take the same sums in three kernels (statistics, loss, gradient) with the statistics all-reduced in between.
 The reference has no distillation loss; the layout follows its vocab-parallel cross-entropy
 (``steptronoss/core/tensor_parallel/cross_entropy.py:28-166``).
@@ -209,7 +209,7 @@ def _grad_kernel(x, ids, t, temperature, weights, stats, grad, vocab_start=0, vo
 
 
 def _whole_rows(x, vocab_start: int, group) -> bool:
-    """Whether the one-pass kernel takes these rows: the whole vocabulary, in the shared memory of a cluster."""
+    """Whether the one-pass kernel takes these rows: the whole vocabulary, of a length that a cluster takes."""
     return vocab_start == 0 and (group is None or _group_size(group) == 1) and _fits_row(x.shape[1], x.element_size())
 
 
