@@ -12,7 +12,7 @@
 //                         (optionally) the gradient, which may overwrite the logits
 //   distill_stats_kernel  a row of any length, or the local part of a vocabulary that is sharded over ranks:
 //                         max, sum of exponentials and the student's logits at the teacher's ids
-//   distill_grad_kernel   the gradient from finished statistics (backward pass; sharded or very long rows)
+//   distill_grad_kernel   the gradient from finished statistics (backward pass of few rows; sharded or very long rows)
 //
 // Statistics of a row: {top, sum, max t, sum of exp((t - max t) / tau)}.  With c = log2(e) / tau, `top` is the rounded
 // c * max s and `sum` that of 2^(c s - top), so that c * max s is rounded once and cancels; the last number is 0 for a
