@@ -1083,6 +1083,19 @@ static long long max_granules(int V, int n) { return (static_cast<long long>(V) 
 constexpr int kRowSmem = 224 * 1024;               // dynamic shared memory of an SM that the row kernel counts on
 constexpr int kRowSlice = 144 * 1024;              // largest slice: 1024 entries, bitmaps and barriers fit beside it
 
+// Shared memory beside the ring, and the chunks of a ring with this many CTAs on an SM.
+static int row_side(int K, int per, int n, bool gradient) {
+  return 2 * (entry_bytes((K + 3) & ~3) + (gradient ? bitmap_bytes(per, n) : 0));
+}
+static int row_ring(int side, int ctas) {
+  const int ring = (kRowSmem / ctas - 2048 - side) / (kChunk * 16);
+  return ring < kMaxChunks ? ring : kMaxChunks;
+}
+// Whether one CTA can pass through a whole row and has room for its entries and bitmaps.
+static bool one_cta_streams(int V, int K, int n) {
+  return row_ring(row_side(K, static_cast<int>(max_granules(V, n)), n, true), 1) >= 2;
+}
+
 template <typename T, typename TO, int C>
 static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   constexpr int n = Lane<T>::n;
@@ -1090,13 +1103,9 @@ static cudaError_t launch_row(const DistillParams& p, cudaStream_t stream) {
   plan.per = static_cast<int>((max_granules(p.V, n) + C - 1) / C);
   plan.chunks = (plan.per + kChunk - 1) / kChunk;
   plan.kpad = (p.K + 3) & ~3;
-  const int side = 2 * (entry_bytes(plan.kpad) + (p.grad != nullptr ? bitmap_bytes(plan.per, n) : 0));
+  const int side = row_side(p.K, plan.per, n, p.grad != nullptr);
   // two CTAs per SM where that leaves each a ring of two chunks, so that one computes while the other waits; else one CTA
-  for (int ctas = 2; ctas >= 1; --ctas) {
-    plan.ring = (kRowSmem / ctas - 2048 - side) / (kChunk * 16);
-    if (plan.ring >= 2) break;
-  }
-  if (plan.ring > kMaxChunks) plan.ring = kMaxChunks;
+  plan.ring = row_ring(side, 2) >= 2 ? row_ring(side, 2) : row_ring(side, 1);
   if (plan.ring < 2) return cudaErrorInvalidValue;
   plan.keep = plan.chunks < plan.ring ? plan.chunks : plan.ring;
   const int smem = plan.ring * kChunk * 16 + side;
@@ -1226,7 +1235,8 @@ extern "C" int stb_distill_grad(const void* logits, long long ld, void* grad, lo
   p.teacher = teacher; p.ld_t = ld_t; p.weight = weight; p.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
   p.T = T; p.V = V; p.K = K; p.vocab_start = vocab_start; p.vocab_total = vocab_total; p.inv_tau = inv_tau;
   if (!distill_args_ok(p) || grad == nullptr || !distill_types_ok(elem_bytes, grad_bytes)) return -kErrBadArgument;
-  if (logits != grad && vocab_start == 0 && vocab_total == V && V <= stb_distill_row_limit(elem_bytes) && many_rows(T)) {
+  if (logits != grad && vocab_start == 0 && vocab_total == V && many_rows(T) &&
+      one_cta_streams(V, K, 16 / elem_bytes)) {
     p.given = p.stats;
     p.stats = nullptr;
     p.status = status;

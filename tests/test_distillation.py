@@ -499,6 +499,31 @@ def test_the_longest_row_of_the_one_pass_kernel_with_the_most_entries(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V,K", [(torch.bfloat16, 400001, 1024), (torch.bfloat16, 585000, 1024), (torch.float32, 290001, 40)])
+def test_many_long_rows(dtype, V, K):
+    """One CTA per row as long as its bitmaps leave room for a ring, and the kernel behind it."""
+    from steptronoss_b200.ops import native, topk_distillation
+
+    T, rows = 300, [0, 150, 299]
+    logits, ids, teacher, w = make(len(rows), V, K, seed=13, dtype=dtype, device="cuda")
+    ids[1, 5], ids[1, 6], ids[2, 0] = 7, 7, V - 1
+    all_x = torch.zeros(T, V, dtype=dtype, device="cuda")
+    all_x[rows] = logits
+    all_ids, all_t, all_w = ids.repeat(100, 1), teacher.repeat(100, 1), torch.ones(T, device="cuda")
+    all_ids[rows], all_t[rows], all_w[rows] = ids, teacher, w
+    tok = topk_distillation(all_x.requires_grad_(), all_ids, all_t)
+    (grad,) = torch.autograd.grad(tok, all_x, all_w)
+    torch.cuda.synchronize()
+    native.raise_if_kernel_error()
+    want, wgrad, p, q = oracle(logits, ids, teacher, 1.0, weights=w)
+    loss_tol, grad_tol = bounds(logits.cpu(), teacher.cpu(), 1.0, p, q, wgrad, w.double().cpu(), dtype)
+    # one CTA adds V / 1024 exponentials into each of a thread's four sums, 572 at most: 400 more than the bound's 200
+    more = 400 * 2.0 ** -24
+    assert (tok.detach()[rows].double().cpu() - want).abs().max() <= loss_tol + more
+    assert ((grad[rows].double().cpu() - wgrad).abs() <= grad_tol + w.double().cpu()[:, None] * p * more).all()
+
+
+@pytest.mark.gpu
 def test_more_elements_than_32_bits_count():
     from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
 
