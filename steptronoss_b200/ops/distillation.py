@@ -414,8 +414,8 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
 
     The counterpart of ``fused_linear_cross_entropy`` for a teacher: ``weights`` holds the loss mask already divided by
     its normaliser (and times ``temperature ** 2`` where the recipe wants that), so the returned scalar is what
-    ``backward()`` is called on; with ``w.main_grad`` the weight gradient is added there during the forward pass.
-    The per-token loss carries no gradient."""
+    ``backward()`` is called on; with ``w.main_grad`` the weight gradient is added there during the forward pass, unless
+    gradients are switched off (``torch.no_grad()``): then only the losses are computed.  The per-token loss carries no gradient."""
     what = "fused_linear_topk_distillation"
     temperature = float(temperature)
     if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1]:
@@ -427,6 +427,11 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
         raise ValueError(f"{what}: h on {h.device}, w on {w.device}")
     ids, t = _checked(h.shape[0], h.get_device(), teacher_ids, teacher_logits, temperature, what)
     wt = _token_weights(weights, h.shape[0], h.get_device(), what)
+    if torch.is_grad_enabled():
+        if weights.requires_grad:
+            raise ValueError(f"{what}: no gradient flows to the weights, detach them")
+    else:
+        h, w = h.detach(), w.detach()        # a Function is told that they need gradients in any mode: main_grad stays as it is
     if not h.is_cuda:
         loss = topk_distillation(torch.nn.functional.linear(h, w), ids, t, temperature, vocab_start, group)
         return torch.where(wt == 0, 0.0, loss * wt).sum(), loss.detach()

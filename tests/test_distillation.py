@@ -233,6 +233,17 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(loss, logits, create_graph=True)
 
 
+def test_fused_head_refuses_weights_that_want_a_gradient():
+    from steptronoss_b200.ops import fused_linear_topk_distillation
+
+    _, ids, teacher, w = make(3, 64, 2)
+    h, head = torch.zeros(3, 16), torch.zeros(64, 16)
+    with pytest.raises(ValueError, match="no gradient flows to the weights"):
+        fused_linear_topk_distillation(h, head, ids, teacher, w.requires_grad_())
+    with torch.no_grad():
+        fused_linear_topk_distillation(h, head, ids, teacher, w)
+
+
 def test_fused_head_refusals():
     from steptronoss_b200.ops import fused_linear_topk_distillation as f
 
@@ -662,6 +673,25 @@ def test_fused_head_adds_into_main_grad():
     total.backward()
     assert head.grad is None and head.grad_added_to_main_grad
     assert torch.allclose(head.main_grad - 1, plain, rtol=2.0 ** -8, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_fused_head_leaves_main_grad_alone_without_gradients(mode):
+    from steptronoss_b200.ops import fused_linear_topk_distillation
+
+    torch.manual_seed(0)
+    T, H, V, K = 40, 64, 512, 8
+    _, ids, teacher, w = make(T, V, K, seed=9, device="cuda")
+    h = torch.randn(T, H, device="cuda").to(torch.bfloat16).requires_grad_()
+    head = torch.nn.Parameter((torch.randn(V, H, device="cuda") * 0.3).to(torch.bfloat16))
+    head.main_grad = torch.ones(V, H, device="cuda")
+    with mode():
+        total, tok = fused_linear_topk_distillation(h, head, ids, teacher, w, chunk_tokens=32)
+    assert head.main_grad.eq(1).all() and not total.requires_grad and not hasattr(head, "grad_added_to_main_grad")
+    # with gradients the same loss, and then they are there
+    total2, tok2 = fused_linear_topk_distillation(h, head, ids, teacher, w, chunk_tokens=32)
+    assert torch.equal(tok, tok2) and total == total2 and head.main_grad.ne(1).any()
 
 
 @pytest.mark.gpu
