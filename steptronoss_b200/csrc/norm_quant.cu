@@ -71,8 +71,9 @@ __device__ __forceinline__ bool usable(float amax) { return amax >= 6e-36f && am
 __device__ __forceinline__ float scale_of(float amax, float steps) {
   return usable(amax) ? __fdiv_rn(amax, steps) : amax < 6e-36f ? 1.f : __uint_as_float(0x7FC00000u);
 }
-// 1 / scale to within 2 units in the last place: it only decides between neighbouring 8-bit values at their border
-__device__ __forceinline__ float inverse_of(float amax, float steps) { return usable(amax) ? __fdividef(steps, amax) : 0.f; }
+// 1 / scale to within 2 units in the last place: it only decides between neighbouring 8-bit values at their border.  Not
+// __fdividef, which gives 0 for a divisor above 2^126, where bf16 rows may well lie.
+__device__ __forceinline__ float inverse_of(float amax, float steps) { return usable(amax) ? __fdiv_rn(steps, amax) : 0.f; }
 
 // Two fp32 at once: one instruction on this architecture.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {

@@ -334,3 +334,21 @@ def test_gpu_refusals():
         ops.quantize_rows_int8(torch.zeros(3, 16, device="cuda"))
     with pytest.raises(ValueError):
         ops.quantize_rows_int8(torch.zeros(1, 32769, dtype=torch.bfloat16, device="cuda"))
+
+
+LARGE = [8.5e37, 8.6e37, 1.2e38, 3.3895e38]      # around 2^126 and up to the largest bf16
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("K", [8, 129, 1990])
+def test_rows_up_to_the_largest_number(device, K):
+    from steptronoss_b200 import ops
+
+    g = torch.Generator().manual_seed(0)
+    x = torch.rand(len(LARGE), K, generator=g) * 2 - 1
+    x[:, K // 2] = 1.0
+    x = (x * torch.tensor(LARGE)[:, None]).to(torch.bfloat16).to(device)
+    assert x.isfinite().all()
+    q, s = ops.quantize_rows_int8(x)
+    assert q[:, K // 2].eq(127).all()
+    check_quantised(q, s, x)

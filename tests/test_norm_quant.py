@@ -206,3 +206,19 @@ def test_a_student_learns_from_a_frozen_teacher_in_8_bits():
         h.mul_(-1.0)
     graph.replay()
     verify(*out)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3_1x128"])
+def test_rows_up_to_the_largest_number(device, fmt):
+    from steptronoss_b200 import ops
+
+    g = torch.Generator().manual_seed(0)
+    # values of one size, so that y = +-w (1 + at most 0.5) stays below 3.4e38
+    x = ((torch.rand(3, 256, generator=g) + 1) * (torch.randint(0, 2, (3, 256), generator=g) * 2 - 1)).to(torch.bfloat16)
+    w = ((torch.rand(256, generator=g) + 1) * 1e38).to(torch.bfloat16)
+    x, d, w = x.to(device), torch.zeros_like(x).to(device), w.to(device)
+    _, y = exact(x, d, w, 1e-6)
+    assert 2.0 ** 126 < y.abs().amax() < 3.3e38
+    _, q, sc = ops.add_rmsnorm_quant(x, d, w, fmt=fmt)
+    (check_quantised if fmt == "int8" else check_e4m3)(q, sc, y, *([256 * U] if fmt == "int8" else []))
