@@ -18,6 +18,12 @@
 // c * max s and `sum` that of 2^(c s - top), so that c * max s is rounded once and cancels; the last number is 0 for a
 // row without entries.  All sums are fp32; the logits' gradient is rounded once.
 //
+// Large rows.  The rounding of c * max s cancels as long as 2 to its power is in range, and c * s may leave the range
+// altogether (a row masked with the type's lowest value).  From |c max s| = 2^31 on neighbouring numbers of that size are
+// 128 apart in the exponent, so that p is the same for all elements that equal the maximum and 0 elsewhere: the exponent
+// is then taken with a power of two instead of c, for which products and differences are exact.  In the statistics such a
+// row, and wherever sums are joined such a part of one, has {max s, -(number of elements that equal it)}.
+//
 // Memory bound: the logits are read once and the gradient written once; two exponentials per element.
 #include "common.cuh"
 
@@ -142,8 +148,66 @@ __device__ __forceinline__ void store_granule(TO* row, int g, int lead, int V, b
   }
 }
 
+// The exponents of a row: fma(s, c, -top).  `sum` is negative for a large row or part of one, whose `top` is its maximum m:
+// the power of two takes m to [2^31, 2^32) (m is above 2^31 / c > 2^10, so that it is a normal number).
+constexpr float kLarge = 2147483648.f;
+struct Exponent { float c, top; };
+__device__ __forceinline__ Exponent exponent_of(float top, float& sum, float c) {
+  if (!(sum < 0.f)) return {c, top};
+  sum = -sum;
+  const float pw = __uint_as_float((285u - ((__float_as_uint(top) >> 23) & 255u)) << 23);
+  return {pw, top * pw};
+}
+// log2 of 2^(c (s - max)), times 2^-32, so that no finite logit leaves the range.
+constexpr float kDown = 1.f / 4294967296.f;
+__device__ __forceinline__ float log_weight(float s, float c, const Exponent& e) {
+  if (e.c == c) return fmaf(s * kDown, c, -e.top * kDown);
+  return (s * kDown - e.top * __frcp_rn(e.c) * kDown) * c;
+}
+
+// (top, sum) of a thread's logits whose largest scaled one is outside (-2^31, 2^31), from another look at them.
+template <typename T>
+struct LargePart {
+  float m = -INFINITY, equal = 0.f;
+  bool bad = false;
+  __device__ __forceinline__ void add(float x) {
+    bad |= x != x;
+    if (x > m) { m = x; equal = 0.f; }
+    if (x == m) equal += 1.f;
+  }
+  __device__ __forceinline__ void add(const uint4& u) {
+    float f[Lane<T>::n];
+    Lane<T>::widen(u, f);
+#pragma unroll
+    for (int j = 0; j < Lane<T>::n; ++j) add(f[j]);
+  }
+  __device__ __forceinline__ void result(float& top, float& sum) const {
+    top = m;                                       // infinite logits are not scaled
+    sum = bad || m == INFINITY ? __uint_as_float(0x7FC00000u) : m == -INFINITY ? 0.f : -equal;
+  }
+};
+
+// Large parts beside others.  `keys`: c * max (infinite for a large part) and a large part's maximum; their maxima over the
+// parts say what the whole is and what each part adds to it.
+__device__ __forceinline__ float2 large_keys(float m, float s) {
+  return s < 0.f ? make_float2(copysignf(INFINITY, m), m) : make_float2(m, -INFINITY);
+}
+__device__ __forceinline__ bool large_whole(float2 keys) { return isinf(keys.x) && keys.y > -INFINITY; }
+__device__ __forceinline__ float large_part(float m, float s, float2 keys) {
+  if (s != s) return s;                            // a NaN stays visible
+  if (large_whole(keys)) return s < 0.f && m == keys.y ? -s : 0.f;
+  return s < 0.f || m == -INFINITY ? fmaxf(s, 0.f) : s * ex2(m - keys.x);
+}
+
 // (m, s) <- the pair that stands for both, s being relative to exp2(m).  -inf: nothing seen yet.
 __device__ __forceinline__ void merge(float& m, float& s, float om, float os) {
+  if (s < 0.f || os < 0.f) {
+    const float2 a = large_keys(m, s), b = large_keys(om, os), keys = make_float2(fmaxf(a.x, b.x), fmaxf(a.y, b.y));
+    s = large_part(m, s, keys) + large_part(om, os, keys);
+    m = large_whole(keys) ? keys.y : keys.x;
+    if (large_whole(keys)) s = -s;
+    return;
+  }
   const float top = fmaxf(m, om);
   const float a = m == top ? s : s * ex2(m - top);
   const float b = om == top ? os : os * ex2(om - top);
@@ -158,11 +222,23 @@ __device__ __forceinline__ float warp_top(float v) {
   return r;
 }
 __device__ __forceinline__ void warp_merge(float& m, float& s) {
-  const float top = warp_top(m);
-  if (m != top) s *= ex2(m - top);
+  float top;
+  const bool large = __any_sync(0xffffffffu, s < 0.f);
+  bool whole = false;
+  if (large) {
+    float2 keys = large_keys(m, s);
+    keys = make_float2(warp_top(keys.x), warp_top(keys.y));
+    whole = large_whole(keys);
+    s = large_part(m, s, keys);
+    top = whole ? keys.y : keys.x;
+  } else {
+    top = warp_top(m);
+    if (m != top) s *= ex2(m - top);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   m = top;
+  if (whole) s = -s;
 }
 
 // Teacher entries of a row in shared memory (statistics and gradient kernels).
@@ -215,12 +291,10 @@ __device__ __forceinline__ void load_entries(const DistillParams& p, const T* ro
   if (lane == 0) { e.tmax = tmax; e.tsum = tsum; }
 }
 
-// One term q (log2 q - log2 p) of the loss, the difference of logarithms taken before the sum over the entries, so
-// that a small divergence is not the difference of two large sums.
-__device__ __forceinline__ float loss_term(float q, float t, float s, float c, const float4& st, float log_sum,
-                                           float log_tsum) {
-  if (q == 0.f) return 0.f;
-  return q * (((t - st.z) * c - log_tsum) - (fmaf(s, c, -st.x) - log_sum));
+// One term q (log2 q - log2 p) of the loss, times 2^-32, the difference of logarithms taken before the sum over the
+// entries, so that a small divergence is not the difference of two large sums.
+__device__ __forceinline__ float loss_term(float q, float log_q, float s, float c, const Exponent& e, float log_sum) {
+  return q == 0.f ? 0.f : q * (log_q * kDown - (log_weight(s, c, e) - log_sum * kDown));
 }
 __device__ __forceinline__ float warp_total(float v) {
 #pragma unroll
@@ -231,9 +305,9 @@ __device__ __forceinline__ float warp_total(float v) {
 // Gradient at the entries: written once more over the dense p, from the logit kept in shared memory, with the q of equal
 // ids added in order.  The caller has a barrier between the dense writes and this.
 template <typename TO>
-__device__ __forceinline__ void write_entries(const DistillParams& p, const Entries& e, TO* grad_row, const float4& st,
-                                              float w) {
-  const float c = p.inv_tau * kLog2e, g = w * p.inv_tau, inv = __fdiv_rn(1.f, st.y);
+__device__ __forceinline__ void write_entries(const DistillParams& p, const Entries& e, TO* grad_row, const Exponent& ex,
+                                              float sum, float w) {
+  const float g = w * p.inv_tau, inv = __fdiv_rn(1.f, sum);
   for (int j = threadIdx.x; j < p.K; j += blockDim.x) {
     const int id = e.id[j];
     if (id < 0) continue;
@@ -244,7 +318,7 @@ __device__ __forceinline__ void write_entries(const DistillParams& p, const Entr
       if (i < j) { first = false; break; }
       q += e.q[i];
     }
-    if (first) Lane<TO>::store(grad_row + id, (ex2(fmaf(e.s[j], c, -st.x)) * inv - q) * g);
+    if (first) Lane<TO>::store(grad_row + id, (ex2(fmaf(e.s[j], ex.c, -ex.top)) * inv - q) * g);
   }
 }
 
@@ -713,23 +787,24 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         failed = 1;
         break;
       }
-      const float top = hd.top, sum = hd.sum;
+      float sum = hd.sum;
+      const Exponent ex = exponent_of(hd.top, sum, c);
       if (rank == 0) {
         if (p.loss != nullptr) {
           const float log_sum = log2f(sum);
           float l = 0.f;
           for (int j = lane; j < p.K; j += 32)
-            l += eq[j] == 0.f ? 0.f : eq[j] * (elq[j] - (fmaf(es[j], c, -top) - log_sum));
+            l += loss_term(eq[j], elq[j], es[j], c, ex, log_sum);
           l = warp_total(l) * kLn2;
-          if (lane == 0) p.loss[row] = l;
+          if (lane == 0) p.loss[row] = l / kDown;
         }
-        if (p.stats != nullptr && lane == 0) p.stats[row] = make_float4(top, sum, tmax, tsum);
+        if (p.stats != nullptr && lane == 0) p.stats[row] = make_float4(hd.top, hd.sum, tmax, tsum);
       }
       if (p.grad != nullptr && w != 0.f) {
         TO* dst = static_cast<TO*>(p.grad) + row * p.ldg;
         const float rs = __fdiv_rn(1.f, sum), gw = w * p.inv_tau;
         for (int j = lane; j < own; j += 32)
-          if (!(gq[j] < 0.f)) Lane<TO>::store(dst + oid[j], (ex2(fmaf(os[j], c, -top)) * rs - gq[j]) * gw);
+          if (!(gq[j] < 0.f)) Lane<TO>::store(dst + oid[j], (ex2(fmaf(os[j], ex.c, -ex.top)) * rs - gq[j]) * gw);
       }
       __syncwarp();
       phase ^= 1;
@@ -822,6 +897,13 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         float sum1;
         unpair(add2(acc[0], acc[1]), sum, sum1);
         sum += sum1;
+        if (!(fabsf(top) < kLarge)) {                 // once more, and nobody has written over the logits yet
+          LargePart<T> again;
+          for (int g = sl.g0 + static_cast<int>(threadIdx.x); g < sl.ge; g += kRowCompute)
+            if (g >= sl.gs) again.add(load_granule<T>(src, g, gr.lead, p.V));
+          again.add(x_edge);
+          again.result(top, sum);
+        }
         warp_merge(top, sum);
         // the logits at the entries have been read: only now may another CTA overwrite them
         ok = ok && mbar_wait_soon(&bars.e_full[b], phase);
@@ -850,10 +932,11 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         TO* dst = static_cast<TO*>(p.grad) + row * p.ldg;
         const bool aligned = granules_aligned<TO, n>(dst, gr.lead);
         const float w = head[b].weight;
+        const Exponent ex = exponent_of(top, sum, c);
         // no entries, or a token that does not count: zero whatever the logits hold
         const bool zero = head[b].tsum == 0.f || w == 0.f;
         const float scale = w * p.inv_tau * __fdiv_rn(1.f, sum);
-        const uint64_t scale2 = pair(scale, scale), minus = pair(-top, -top);
+        const uint64_t scale2 = pair(scale, scale), minus = pair(-ex.top, -ex.top), cx = pair(ex.c, ex.c);
         TO* out = dst - gr.lead;
         if (zero) {
           const uint64_t none[kP] = {};
@@ -864,7 +947,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           uint64_t f[kP];
           Pairs<T>::widen(v, f);
 #pragma unroll
-          for (int j = 0; j < kP; ++j) f[j] = mul2(ex2_2(fma2(f[j], c2, minus)), scale2);
+          for (int j = 0; j < kP; ++j) f[j] = mul2(ex2_2(fma2(f[j], cx, minus)), scale2);
           store_pairs<TO, kP>(out + granule * n, aligned, f);
         };
         auto finish = [&](int k, int at) {            // chunk k of the slice, at this place of the ring
@@ -903,7 +986,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
           }
         }
         if (!ok) { leave(); break; }
-        if (edge >= 0) Lane<TO>::store(dst + edge, zero ? 0.f : ex2(fmaf(x_edge, c, -top)) * scale);
+        if (edge >= 0) Lane<TO>::store(dst + edge, zero ? 0.f : ex2(fmaf(x_edge, ex.c, -ex.top)) * scale);
       }
       mbar_arrive_warp(&bars.e_empty[b]);
     }
@@ -959,6 +1042,11 @@ distill_stats_kernel(const DistillParams p) {
       for (int j = 0; j < n; ++j) sum += ex2(fmaf(f[j], c, -base));
     }
   }
+  if (!(fabsf(top) < kLarge)) {
+    LargePart<T> again;
+    for (int g = threadIdx.x; g < gr.count; g += kDsStatsThreads) again.add(load_granule<T>(src, g, gr.lead, p.V));
+    again.result(top, sum);
+  }
   block_merge<kDsStatsThreads>(top, sum, red);
   if (threadIdx.x == 0) p.stats[row] = make_float4(top, sum, e.tmax, e.tsum);
 }
@@ -971,18 +1059,20 @@ distill_loss_kernel(const DistillParams p) {
   if (row >= p.T) return;
   const float c = p.inv_tau * kLog2e;
   const float4 st = p.stats[row];
+  float sum = st.y;
+  const Exponent ex = exponent_of(st.x, sum, c);
   float l = 0.f;
   if (st.w != 0.f) {
-    const float inv = __fdiv_rn(1.f, st.w), log_sum = log2f(st.y), log_tsum = log2f(st.w);
+    const float inv = __fdiv_rn(1.f, st.w), log_sum = log2f(sum), log_tsum = log2f(st.w);
     for (int j = lane; j < p.K; j += 32) {
       const long long id = entry_id(p, row, j);
       if (id < 0 || id >= p.vocab_total) continue;
       const float t = p.teacher[row * p.ld_t + j];
-      l += loss_term(entry_q(t, st.z, inv, c), t, p.picked[row * p.K + j], c, st, log_sum, log_tsum);
+      l += loss_term(entry_q(t, st.z, inv, c), (t - st.z) * c - log_tsum, p.picked[row * p.K + j], c, ex, log_sum);
     }
   }
   l = warp_total(l) * kLn2;
-  if (lane == 0) p.loss[row] = l;
+  if (lane == 0) p.loss[row] = l / kDown;
 }
 
 // ------------------------------------------------------------------------------------------- gradient from statistics
@@ -1004,6 +1094,8 @@ distill_grad_kernel(const DistillParams p, int chunks) {
   const float w = p.weight != nullptr ? p.weight[row] : 1.f;
   const bool zero = st.w == 0.f || w == 0.f;
   const float c = p.inv_tau * kLog2e;
+  float sum = st.y;
+  const Exponent ex = exponent_of(st.x, sum, c);
   uint4 v[kGradVec];
   if (!zero) {
 #pragma unroll
@@ -1024,7 +1116,7 @@ distill_grad_kernel(const DistillParams p, int chunks) {
     }
     __syncthreads();
   }
-  const float g = w * p.inv_tau * __fdiv_rn(1.f, st.y);
+  const float g = w * p.inv_tau * __fdiv_rn(1.f, sum);
 #pragma unroll
   for (int i = 0; i < kGradVec; ++i) {
     const int k = g0 + i * kDsThreads + threadIdx.x;
@@ -1032,12 +1124,12 @@ distill_grad_kernel(const DistillParams p, int chunks) {
     float f[n];
     if (!zero) Lane<T>::widen(v[i], f);
 #pragma unroll
-    for (int j = 0; j < n; ++j) f[j] = zero ? 0.f : ex2(fmaf(f[j], c, -st.x)) * g;
+    for (int j = 0; j < n; ++j) f[j] = zero ? 0.f : ex2(fmaf(f[j], ex.c, -ex.top)) * g;
     store_granule<TO, n>(dst, k, gr.lead, p.V, aligned, f);
   }
   if (zero) return;
   __syncthreads();
-  write_entries<TO>(p, e, dst, st, w);
+  write_entries<TO>(p, e, dst, ex, sum, w);
 }
 
 // ------------------------------------------------------------------------------------------- fused head: total, scaling

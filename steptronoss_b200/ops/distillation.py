@@ -104,25 +104,29 @@ def _teacher_q(ids, t, temperature: float, vocab: int):
     if t.shape[-1] == 0:
         return t, t, torch.zeros(t.shape[0], dtype=torch.bool, device=t.device)
     has = entry.any(-1)
-    t = torch.where(entry, t, -math.inf) / temperature
-    logq = torch.log_softmax(torch.where(has.unsqueeze(-1), t, 0.0), dim=-1)
+    t = torch.where(entry, t, -math.inf)
+    t = torch.where(has.unsqueeze(-1), (t - t.amax(-1, keepdim=True)) / temperature, 0.0)
+    logq = torch.log_softmax(t, dim=-1)
     return torch.where(entry, logq.exp(), 0.0), logq, has
 
 
 def _statement(logits, ids, t, temperature: float, vocab_start: int, group):
-    """``(loss [T], gradient [T, V] for a unit weight)`` in fp32 (fp64 for fp64 logits) from (a vocab shard of) the logits."""
-    s = (logits if logits.dtype == torch.float64 else logits.float()) / temperature
+    """``(loss [T], gradient [T, V] for a unit weight)`` in fp32 (fp64 for fp64 logits) from (a vocab shard of) the logits.
+
+    The maximum is subtracted before the division: logits of the type's lowest value are finite and stay so.  The few
+    numbers of an entry's loss are taken in fp64, where differences of such logits are finite, too."""
+    s = logits if logits.dtype == torch.float64 else logits.float()
     V = s.shape[-1]
     q, logq, has = _teacher_q(ids, t.to(s.dtype), temperature, V * _group_size(group))
     top = _all_reduce(s.amax(-1), dist.ReduceOp.MAX, group)
-    e = (s - top.unsqueeze(-1)).exp()
+    e = ((s - top.unsqueeze(-1)) / temperature).exp()
     total = _all_reduce(e.sum(-1), dist.ReduceOp.SUM, group)
     local = ids - vocab_start
     here = (local >= 0) & (local < V) & (q != 0)
     safe = local.masked_fill(~here, 0).long()
     picked = _all_reduce(torch.where(here, s.gather(-1, safe), 0.0), dist.ReduceOp.SUM, group)
-    terms = q * (logq - (picked - top.unsqueeze(-1) - total.log().unsqueeze(-1)))
-    loss = torch.where(q != 0, terms, 0.0).sum(-1)
+    logp = (picked.double() - top.double().unsqueeze(-1)) / temperature - total.double().log().unsqueeze(-1)
+    loss = torch.where(q != 0, q.double() * (logq.double() - logp), 0.0).sum(-1).to(s.dtype)
     grad = (e / total.unsqueeze(-1)).scatter_add(-1, safe, -torch.where(here, q, 0.0)) / temperature
     return loss, torch.where(has.unsqueeze(-1), grad, 0.0)
 
@@ -184,14 +188,33 @@ def _stats_kernels(x, ids, t, temperature, vocab_start=0, group=None, loss=None)
     return loss, stats
 
 
+def _shard_keys(stats):
+    """``[2, T]``, whose maxima over the shards are the whole rows': ``c * max`` (infinite for large rows, which have a
+    negative sum) and the maximum of large rows itself."""
+    top, large = stats[:, 0], stats[:, 1] < 0
+    return torch.stack([torch.where(large, torch.copysign(torch.full_like(top, math.inf), top), top),
+                        torch.where(large, top, -math.inf)])
+
+
+def _shard_sums(stats, keys):
+    """A shard's sums relative to the maxima of the whole rows, and which of these are large."""
+    (top, total), large = (stats[:, 0], stats[:, 1]), stats[:, 1] < 0
+    rows = keys[0].isinf() & (keys[1] != -math.inf)
+    # a shard that holds nothing but -inf has top = -inf and sum 0; beside a large one only equal maxima count
+    usual = torch.where(top == -math.inf, total, total * torch.exp2(top - keys[0]))
+    sums = torch.where(rows, torch.where(large & (top == keys[1]), -total, 0.0), torch.where(large, 0.0, usual))
+    return torch.where(total.isnan(), total, sums), rows
+
+
 def _join_shards(stats, picked, group) -> None:
-    """Statistics of whole rows from those of the group's vocabulary shards, in place.  The first two columns are
-    ``(top, sum of 2^(c s - top))``; the teacher's columns are equal on all ranks."""
-    top = _all_reduce(stats[:, 0].clone(), dist.ReduceOp.MAX, group)
-    # a shard that holds nothing but -inf has top = -inf and sum 0
-    scaled = torch.where(stats[:, 0] == -math.inf, stats[:, 1], stats[:, 1] * torch.exp2(stats[:, 0] - top))
-    stats[:, 1] = _all_reduce(scaled, dist.ReduceOp.SUM, group)
-    stats[:, 0] = top
+    """Statistics of whole rows from those of the group's vocabulary shards, in place.  The first two columns are ``(top,
+    sum of 2^(c s - top))``, or for large rows ``(max, -number of elements that equal it)``; the teacher's columns are
+    equal on all ranks."""
+    keys = _all_reduce(_shard_keys(stats), dist.ReduceOp.MAX, group)
+    sums, rows = _shard_sums(stats, keys)
+    sums = _all_reduce(sums, dist.ReduceOp.SUM, group)
+    stats[:, 0] = torch.where(rows, keys[1], keys[0])
+    stats[:, 1] = torch.where(rows, -sums, sums)
     _all_reduce(picked, dist.ReduceOp.SUM, group)
 
 

@@ -755,3 +755,152 @@ def test_gpu_refusals():
         fused_linear_topk_distillation(bf(4, 8), bf(17, 8), ids, teacher, w)
     with pytest.raises(ValueError):
         fused_linear_topk_distillation(bf(4, 12), bf(16, 12), ids, teacher, w)
+
+
+def lowest_rows(T, V, K, dtype, device, tau):
+    """Rows masked with the type's lowest value: in part, an entry among it; throughout; throughout but for -inf; a logit of
+    the type's largest value; entries of a teacher that is masked so; and ordinary rows behind them."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    logits, ids, teacher, w = make(T, V, K, seed=20, dtype=dtype)
+    ids[:, 0] = torch.arange(T) % V
+    for j in range(1, K):                           # distinct ids
+        ids[:, j] = (ids[:, 0] + 1 + 3 * j) % V
+    logits[0, V // 2:] = low
+    logits[0, ids[0, 1]] = low
+    logits[1] = low
+    logits[2] = low
+    logits[2, V // 3:V // 2] = -INF
+    ids[2] = torch.arange(K)
+    logits[3, ids[3, 2]] = high
+    teacher[4, 1:] = torch.finfo(torch.float32).min
+    logits[5, ids[5]] = 0.75 * low                  # all entries masked
+    want, wgrad, p, q = oracle(logits, ids, teacher, tau, weights=w)
+    usual = torch.where(logits.abs() > 1e38, 0.0, logits.float())
+    usual_t = torch.where(teacher < -1e38, 0.0, teacher)
+    # logits of that size leave p = 0 or equal parts: exponents are 0 or far below the range.  The other terms are those of
+    # `bounds`; a loss of that size is q times a difference, off by less than loss_tol of itself
+    loss_tol, grad_tol = bounds(usual, usual_t, tau, p, q, wgrad, w.double(), dtype)
+    big = torch.finfo(torch.float32).max
+    assert ((want - big).abs() > 1e-3 * big).all()
+
+    def verify(loss, grad):
+        loss = loss.double().cpu()
+        assert loss[want > big].eq(INF).all()
+        fine = want < big
+        assert ((loss - want)[fine].abs() <= loss_tol * (1 + want[fine].abs())).all(), (loss[:6], want[:6])
+        assert ((grad.double().cpu() - wgrad).abs() <= grad_tol).all()
+
+    return [t.to(device) for t in (logits, ids, teacher, w)], verify
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tau", [0.5, 1.0, 2.0])
+@pytest.mark.parametrize("T,V,K", [(6, 40, 3), (7, 5003, 12)])
+def test_logits_masked_with_the_lowest_value(device, dtype, tau, T, V, K):
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    (logits, ids, teacher, w), verify = lowest_rows(T, V, K, dtype, device, tau)
+    verify(*topk_distillation_loss_and_grad(logits, ids, teacher, w, tau))
+    x = logits.clone().requires_grad_()
+    tok = topk_distillation(x, ids, teacher, tau)
+    verify(tok.detach(), torch.autograd.grad(tok, x, w)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,T,V", [(torch.bfloat16, 310, 3001), (torch.float32, 310, 3001),     # one CTA per row
+                                       (torch.bfloat16, 6, 151936), (torch.float32, 6, 151936),     # clusters
+                                       (torch.bfloat16, 6, 600001), (torch.float32, 6, 300001)])    # three kernels
+def test_logits_masked_with_the_lowest_value_in_every_kernel(dtype, T, V):
+    from steptronoss_b200.ops import native, topk_distillation, topk_distillation_loss_and_grad
+
+    (logits, ids, teacher, w), verify = lowest_rows(T, V, 9, dtype, "cuda", 1.0)
+    verify(*topk_distillation_loss_and_grad(logits, ids, teacher, w))
+    x = logits.clone().requires_grad_()
+    tok = topk_distillation(x, ids, teacher)
+    verify(tok.detach(), torch.autograd.grad(tok, x, w)[0])
+    torch.cuda.synchronize()
+    native.raise_if_kernel_error()
+
+
+def test_statistics_of_large_rows_are_joined():
+    """Rows by what their two shards hold: (top, sum), for large rows (max, -count)."""
+    from steptronoss_b200.ops.distillation import _shard_keys, _shard_sums
+
+    low, cases = -3.4e38, []
+    cases.append(((5.0, 2.0), (3.0, 4.0), (5.0, 3.0)))                  # ordinary: 2 + 4 / 4
+    cases.append(((-INF, 0.0), (3.0, 4.0), (3.0, 4.0)))
+    cases.append(((-INF, 0.0), (-INF, 0.0), (-INF, 0.0)))
+    cases.append(((low, -7.0), (3.0, 4.0), (3.0, 4.0)))                 # masked beside ordinary
+    cases.append(((low, -7.0), (-2e9, 4.0), (-2e9, 4.0)))
+    cases.append(((low, -7.0), (low, -2.0), (low, -9.0)))               # masked throughout
+    cases.append(((low, -7.0), (-2.4e38, -2.0), (-2.4e38, -2.0)))
+    cases.append(((low, -7.0), (-INF, 0.0), (low, -7.0)))
+    cases.append(((3e38, -1.0), (9.0, 4.0), (3e38, -1.0)))
+    cases.append(((3e38, -1.0), (low, -4.0), (3e38, -1.0)))
+    cases.append(((3e38, -1.0), (9.0, math.nan), (3e38, math.nan)))     # a NaN stays visible
+    a, b, want = (torch.tensor([c[i] for c in cases]) for i in range(3))
+    keys = torch.maximum(_shard_keys(a), _shard_keys(b))
+    (sa, large), (sb, other) = _shard_sums(a, keys), _shard_sums(b, keys)
+    assert torch.equal(large, other) and torch.equal(large, want[:, 1].lt(0) | want[:, 1].isnan())
+    assert torch.equal(torch.where(large, keys[1], keys[0]), want[:, 0])
+    got = torch.where(large, -(sa + sb), sa + sb)
+    assert torch.allclose(got, want[:, 1], rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("parts", [1, 3])
+def test_shards_with_the_lowest_value_equal_the_whole(dtype, parts):
+    """The kernels of a sharded vocabulary on logits masked with the type's lowest value."""
+    from steptronoss_b200.ops import distillation as d
+    from steptronoss_b200.ops import native
+
+    T, V, K, tau = 7, 3000, 9, 0.5
+    (logits, ids, teacher, w), verify = lowest_rows(T, V, K, dtype, "cuda", tau)
+    lib, st, width = native.load(), native.stream(), V // parts
+    stats, picked = [], []
+    for r in range(parts):
+        x = logits[:, r * width:(r + 1) * width]
+        stats.append(torch.empty(T, 4, device="cuda"))
+        picked.append(torch.empty(T, K, device="cuda"))
+        assert lib.stb_distill_stats(x.data_ptr(), x.stride(0), ids.data_ptr(), 1, ids.stride(0), teacher.data_ptr(), K,
+                                     stats[r].data_ptr(), picked[r].data_ptr(), T, width, K, r * width, V, 1 / tau,
+                                     x.element_size(), st) == 0
+    keys = torch.stack([d._shard_keys(s) for s in stats]).amax(0)
+    sums = sum(d._shard_sums(s, keys)[0] for s in stats)
+    large = d._shard_sums(stats[0], keys)[1]
+    whole = stats[0].clone()
+    whole[:, 0], whole[:, 1] = torch.where(large, keys[1], keys[0]), torch.where(large, -sums, sums)
+    together, loss, grad = sum(picked), torch.empty(T, device="cuda"), torch.empty_like(logits)
+    assert lib.stb_distill_loss(ids.data_ptr(), 1, ids.stride(0), teacher.data_ptr(), K, whole.data_ptr(),
+                                together.data_ptr(), loss.data_ptr(), T, K, V, 1 / tau, st) == 0
+    for r in range(parts):
+        sl = slice(r * width, (r + 1) * width)
+        d._grad_kernel(logits[:, sl], ids, teacher, tau, w, whole, grad[:, sl], r * width, V)
+    verify(loss, grad)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 3e9, 1e12, 1e30])
+def test_logits_of_any_size(device, size):
+    """Rows whose numbers all lie near `size`, a few units in the last place apart, on both sides of zero."""
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    T, V, K = 4, 700, 5
+    g = torch.Generator().manual_seed(23)
+    base = torch.tensor([size, -size, size, -size])[:, None].expand(T, V).contiguous()
+    logits = base.view(torch.int32).add(torch.randint(0, 4, (T, V), generator=g, dtype=torch.int32)).view(torch.float32)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(T)])
+    teacher, w = torch.randn(T, K, generator=g), torch.ones(T)
+    for tau in (0.25, 1.0, 3.0):
+        loss, grad = topk_distillation_loss_and_grad(*(t.to(device) for t in (logits, ids, teacher, w)), tau)
+        want, wgrad, p, q = oracle(logits, ids, teacher, tau)
+        # only differences from the maximum count, and they are exact; the rounding of c * max s, half a unit in its last
+        # place, cancels, but passes through one sum and one logarithm of its size
+        near = logits - logits.amax(1, keepdim=True)
+        loss_tol, grad_tol = bounds(near, teacher, tau, p, q, wgrad, w.double(), torch.float32)
+        more = 4 * min(1.4427 * size / tau, 2.0 ** 31) * 2.0 ** -48
+        assert ((loss.double().cpu() - want).abs() <= loss_tol * (1 + want) + more).all()
+        # beside large maxima what lies 64 or more below in the exponent may count as nothing
+        assert ((grad.double().cpu() - wgrad).abs() <= grad_tol + (p * more + 2.0 ** -64) / tau).all()
