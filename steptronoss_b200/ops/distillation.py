@@ -26,7 +26,7 @@ import torch.distributed as dist
 
 from . import native
 from .cross_entropy import _all_reduce
-from .gemm import count_launch, gemm
+from .gemm import _tma_compatible, count_launch, gemm
 
 MAX_ENTRIES = 1024
 P, I, L, F = native.P, native.I, native.L, native.F
@@ -365,10 +365,12 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
         V = w.shape[0]
         need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         main_grad = getattr(w, "main_grad", None) if need_dw else None
+        # elsewhere than on 16-byte boundaries the product would be the library's, rounded to bf16 once per block
+        into_main_grad = main_grad is not None and _tma_compatible(main_grad)
         f32 = torch.float32
         loss, total = h.new_empty(T, dtype=f32), h.new_empty((), dtype=f32)
         dh = h.new_empty((T, H), dtype=f32) if need_dh else None
-        dw = main_grad
+        dw = main_grad if into_main_grad else None
         if need_dw and dw is None:
             dw = h.new_empty((V, H), dtype=f32) if T else h.new_zeros((V, H), dtype=f32)
         rows = min(chunk, T)
@@ -392,7 +394,9 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
             if need_dh:
                 gemm(g, w, b_mn_major=True, out=dh if whole else dh[t0:t0 + n])
             if need_dw:
-                gemm(g, hc, a_mn_major=True, b_mn_major=True, out=dw, accumulate=main_grad is not None or t0 > 0)
+                gemm(g, hc, a_mn_major=True, b_mn_major=True, out=dw, accumulate=into_main_grad or t0 > 0)
+        if main_grad is not None and not into_main_grad:
+            main_grad.add_(dw)
         native.check(native.launch(native.load().stb_distill_total, h.get_device(), loss.data_ptr(), weights.data_ptr(), T,
                                    total.data_ptr()), "distill_total")
         count_launch()
@@ -420,6 +424,11 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
             else:
                 gw = _scaled(ctx.dw, gloss)
         return gh, gw, None, None, None, None, None, None, None
+
+
+def _rows_for_gemm(x: torch.Tensor) -> bool:
+    """Whether the tcgen05 GEMM takes these bf16 rows; it leaves others to a library product that rounds to bf16."""
+    return _tma_compatible(x) and (x.shape[0] < 2 or x.stride(0) >= x.shape[1])
 
 
 def _scaled(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
@@ -462,9 +471,9 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
         raise TypeError(f"{what}: h and w are bf16, got {h.dtype} and {w.dtype}")
     if h.get_device() != torch.cuda.current_device():
         raise ValueError(f"{what}: h is on {h.device}, which is not the current device (the GEMMs go to the current one)")
-    if w.shape[0] % 8 or w.shape[1] % 8 or w.data_ptr() % 16 or w.stride(1) != 1 or w.stride(0) % 8:
-        raise ValueError(f"{what}: w needs a vocabulary and a hidden size that are multiples of 8 and 16-byte aligned "
+    if w.shape[0] % 8 or w.shape[1] % 8 or not _rows_for_gemm(w):
+        raise ValueError(f"{what}: w needs a vocabulary and a hidden size that are multiples of 8 and separate 16-byte aligned "
                          f"rows, got {tuple(w.shape)} with strides {w.stride()}")
-    if h.stride(1) != 1 or h.data_ptr() % 16 or h.stride(0) % 8:
-        h = h.contiguous()
+    if not _rows_for_gemm(h):
+        h = h.clone(memory_format=torch.contiguous_format)     # contiguous() would return a shifted or single row as it is
     return _FusedLinearTopkDistillationFn.apply(h, w, ids, t, wt, temperature, int(vocab_start), group, int(chunk_tokens))

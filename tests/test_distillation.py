@@ -904,3 +904,56 @@ def test_logits_of_any_size(device, size):
         assert ((loss.double().cpu() - want).abs() <= loss_tol * (1 + want) + more).all()
         # beside large maxima what lies 64 or more below in the exponent may count as nothing
         assert ((grad.double().cpu() - wgrad).abs() <= grad_tol + (p * more + 2.0 ** -64) / tau).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["one element off", "single token from an odd pitch", "single token one element off",
+                                 "one row repeated", "rows that overlap", "odd pitch"])
+def test_fused_head_takes_hidden_states_on_any_address(how):
+    """The same numbers whatever the layout: the fp32 logits of the framework's own product."""
+    from steptronoss_b200.ops import fused_linear_topk_distillation
+
+    torch.manual_seed(0)
+    T, H, V, K = 90, 64, 1000, 8
+    if "single" in how:
+        T = 1
+    _, ids, teacher, w = make(T, V, K, seed=21, device="cuda")
+    store = torch.randn(T * (H + 3) + 1, device="cuda").to(torch.bfloat16)
+    h = {"one element off": lambda: store[1:1 + T * H].view(T, H),
+         "single token from an odd pitch": lambda: store[:H + 3].view(1, H + 3)[:, :H],
+         "single token one element off": lambda: store[1:1 + H].view(1, H),
+         "one row repeated": lambda: store[:H].expand(T, H),
+         "rows that overlap": lambda: store.as_strided((T, H), (8, 1)),
+         "odd pitch": lambda: store[:T * (H + 3)].view(T, H + 3)[:, :H]}[how]()
+    head = (torch.randn(V, H, device="cuda") * 0.8).to(torch.bfloat16).requires_grad_()
+
+    def run(x):
+        total, tok = fused_linear_topk_distillation(x, head, ids, teacher, w, chunk_tokens=32)
+        return (total.detach(), tok, *torch.autograd.grad(total, [x, head]))
+
+    want = run(torch.empty(T, H, dtype=h.dtype, device="cuda").copy_(h).requires_grad_())
+    for a, b in zip(run(h.detach().requires_grad_()), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_fused_head_takes_a_main_grad_on_any_address():
+    from steptronoss_b200.ops import fused_linear_topk_distillation
+
+    torch.manual_seed(0)
+    T, H, V, K = 90, 64, 512, 8
+    _, ids, teacher, w = make(T, V, K, seed=8, device="cuda")
+    h = torch.randn(T, H, device="cuda").to(torch.bfloat16)
+    head = torch.nn.Parameter((torch.randn(V, H, device="cuda") * 0.3).to(torch.bfloat16))
+
+    def run(main_grad):
+        head.main_grad = main_grad.fill_(1.0)
+        total, _ = fused_linear_topk_distillation(h, head, ids, teacher, w, chunk_tokens=32)
+        total.backward()
+        assert head.grad is None
+        return head.main_grad
+
+    want = run(torch.empty(V, H, device="cuda"))
+    got = run(torch.empty(V * H + 1, device="cuda")[1:].view(V, H))
+    # three blocks and the 1 that was there, in another order: four roundings of 2^-24 on each side
+    assert ((got - want).abs() <= 8 * 2.0 ** -24 * (1 + (want - 1).abs() * 3)).all()
