@@ -352,3 +352,20 @@ def test_rows_up_to_the_largest_number(device, K):
     q, s = ops.quantize_rows_int8(x)
     assert q[:, K // 2].eq(127).all()
     check_quantised(q, s, x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(2000, 512), (700, 1990), (300, 4096), (9, 20001)])
+def test_values_are_the_nearest_to_the_quotient_by_the_stored_scale(M, K):
+    """bf16 rows are full of quotients that lie on a border between two values (rows whose largest value is a power of two
+    have 63.5 steps at its half), so the division has to be the one that the definition makes."""
+    from steptronoss_b200 import ops
+    from steptronoss_b200.ops.int8 import quantize_rows_int8_reference
+
+    torch.manual_seed(4)
+    x = (torch.randn(M, K, device="cuda") * torch.rand(M, 1, device="cuda").mul(60).sub(30).exp2()).to(torch.bfloat16)
+    x[::3, 5] = x[::3].float().abs().amax(1).log2().ceil().exp2().to(torch.bfloat16)     # largest value a power of two
+    x[::3, 6] = x[::3, 5] / 2
+    q, s = ops.quantize_rows_int8(x)
+    want, ws = quantize_rows_int8_reference(x.cpu())               # where / is a division
+    assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), want)

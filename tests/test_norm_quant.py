@@ -222,3 +222,24 @@ def test_rows_up_to_the_largest_number(device, fmt):
     assert 2.0 ** 126 < y.abs().amax() < 3.3e38
     _, q, sc = ops.add_rmsnorm_quant(x, d, w, fmt=fmt)
     (check_quantised if fmt == "int8" else check_e4m3)(q, sc, y, *([256 * U] if fmt == "int8" else []))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", [(64, 512), (33, 4096), (5, 32768)])
+def test_values_behind_the_norm_are_the_nearest_to_the_quotient(T, H):
+    """With |s| = 1 throughout and eps = 0 the norm is exact: y = +-w."""
+    from steptronoss_b200 import ops
+    from steptronoss_b200.ops.norm_quant import _quantized_e4m3
+    from steptronoss_b200.ops.int8 import quantize_rows_int8_reference
+
+    torch.manual_seed(5)
+    x = torch.randint(0, 2, (T, H), device="cuda").mul(2).sub(1).to(torch.bfloat16)
+    w = (torch.randn(H, device="cuda") * torch.randint(-3, 4, (H,), device="cuda").float().exp2()).to(torch.bfloat16)
+    w[0], w[1] = 32.0, 16.0
+    y = (x.float() * w.float()).cpu()
+    q, s = ops.rmsnorm_quant(x, w, 0.0)
+    want, ws = quantize_rows_int8_reference(y)
+    assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), want)
+    q, s = ops.rmsnorm_quant(x, w, 0.0, fmt="e4m3_1x128")
+    want, ws = _quantized_e4m3(y)
+    assert torch.equal(s.cpu(), ws) and torch.equal(q.float().cpu(), want.float())
