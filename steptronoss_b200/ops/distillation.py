@@ -34,6 +34,7 @@ native.register_signature("stb_distill_row_limit", [I])
 native.register_signature("stb_distill_row", [P, L, P, L, P, I, L, P, L, P, P, P, I, I, I, F, I, I, P, P])
 native.register_signature("stb_distill_stats", [P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, P])
 native.register_signature("stb_distill_loss", [P, I, L, P, L, P, P, P, I, I, L, F, P])
+native.register_signature("stb_distill_live", [P, L, P, I, L, P, L, P, P, I, I, I, L, P])
 native.register_signature("stb_distill_total", [P, P, I, P, P])
 native.register_signature("stb_distill_scale", [P, P, P, L, P])
 native.register_signature("stb_distill_grad", [P, L, P, L, P, I, L, P, L, P, P, I, I, I, L, L, F, I, I, P, P])
@@ -376,6 +377,7 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
         rows = min(chunk, T)
         logits = h.new_empty((rows, V), dtype=f32)
         grad = h.new_empty((rows, V)) if need_dh or need_dw else None
+        live = h.new_empty((rows, H)) if need_dw else None
         for t0 in range(0, T, chunk):
             n = min(T - t0, chunk)
             whole = n == T
@@ -394,7 +396,8 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
             if need_dh:
                 gemm(g, w, b_mn_major=True, out=dh if whole else dh[t0:t0 + n])
             if need_dw:
-                gemm(g, hc, a_mn_major=True, b_mn_major=True, out=dw, accumulate=into_main_grad or t0 > 0)
+                hl = _live_states(hc, *args[1:3], weights if whole else weights[t0:t0 + n], V * _group_size(group), live[:n])
+                gemm(g, hl, a_mn_major=True, b_mn_major=True, out=dw, accumulate=into_main_grad or t0 > 0)
         if main_grad is not None and not into_main_grad:
             main_grad.add_(dw)
         native.check(native.launch(native.load().stb_distill_total, h.get_device(), loss.data_ptr(), weights.data_ptr(), T,
@@ -424,6 +427,17 @@ class _FusedLinearTopkDistillationFn(torch.autograd.Function):
             else:
                 gw = _scaled(ctx.dw, gloss)
         return gh, gw, None, None, None, None, None, None, None
+
+
+def _live_states(h, ids, t, weights, vocab, out):
+    """``h`` into ``out``, with zeros for tokens that do not count: of weight 0, or without an entry."""
+    T, H = h.shape
+    native.check(native.launch(
+        native.load().stb_distill_live, h.get_device(), h.data_ptr(), h.stride(0), ids.data_ptr(),
+        int(ids.dtype == torch.int64), ids.stride(0), t.data_ptr(), t.stride(0), weights.data_ptr(), out.data_ptr(), T, H,
+        ids.shape[1], vocab), "distill_live")
+    count_launch()
+    return out
 
 
 def _rows_for_gemm(x: torch.Tensor) -> bool:
@@ -465,7 +479,11 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
     else:
         h, w = h.detach(), w.detach()        # a Function is told that they need gradients in any mode: main_grad stays as it is
     if not h.is_cuda:
-        loss = topk_distillation(torch.nn.functional.linear(h, w), ids, t, temperature, vocab_start, group)
+        linear = torch.nn.functional.linear
+        entries = (ids >= 0) & (ids < w.shape[0] * _group_size(group)) & (t != -math.inf)
+        live = ((wt != 0) & entries.any(-1)).unsqueeze(-1)
+        logits = torch.where(live, linear(torch.where(live, h, 0.0), w), linear(h, w).detach())
+        loss = topk_distillation(logits, ids, t, temperature, vocab_start, group)
         return torch.where(wt == 0, 0.0, loss * wt).sum(), loss.detach()
     if h.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise TypeError(f"{what}: h and w are bf16, got {h.dtype} and {w.dtype}")

@@ -957,3 +957,38 @@ def test_fused_head_takes_a_main_grad_on_any_address():
     got = run(torch.empty(V * H + 1, device="cuda")[1:].view(V, H))
     # three blocks and the 1 that was there, in another order: four roundings of 2^-24 on each side
     assert ((got - want).abs() <= 8 * 2.0 ** -24 * (1 + (want - 1).abs() * 3)).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("main_grad", [False, True])
+def test_fused_head_passes_over_hidden_states_that_do_not_count(device, main_grad):
+    """Tokens of weight 0 and without entries may hold anything, in their hidden states too."""
+    from steptronoss_b200.ops import fused_linear_topk_distillation
+
+    torch.manual_seed(0)
+    T, H, V, K = 70, 32, 200, 5
+    _, ids, teacher, w = make(T, V, K, seed=22)
+    teacher[3], teacher[40], ids[69] = -INF, -INF, V
+    w[2], w[33] = 0.0, 0.0
+    dead = torch.tensor([2, 3, 33, 40, 69])
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    ids, teacher, w, h = ids.to(device), teacher.to(device), w.to(device), torch.randn(T, H).to(device, dtype)
+    head = torch.nn.Parameter((torch.randn(V, H) * 0.5).to(device, dtype))
+
+    def run(x):
+        x = x.clone().requires_grad_()
+        head.grad = None
+        if main_grad and device == "cuda":
+            head.main_grad = torch.zeros(V, H, device="cuda")
+        total, tok = fused_linear_topk_distillation(x, head, ids, teacher, w, 2.0, chunk_tokens=32)
+        total.backward()
+        return total.detach(), tok, x.grad, head.main_grad if main_grad and device == "cuda" else head.grad
+
+    h[dead] = 0
+    want = run(h)
+    h[dead] = torch.tensor([math.nan, INF, -INF, math.nan, math.nan], dtype=dtype, device=device)[:, None]
+    total, tok, dh, dw = run(h)
+    assert total == want[0] and torch.equal(dw, want[3]) and torch.equal(dh, want[2]) and dh[dead].eq(0).all()
+    live = torch.ones(T, dtype=torch.bool)
+    live[dead] = False
+    assert torch.equal(tok[live], want[1][live]) and tok[[3, 40, 69]].eq(0).all()
