@@ -435,6 +435,8 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   const uint32_t tmem_base = *tmem_slot;
   wait_for_previous_kernel();
   let_next_kernel_start();
+  // The scales are read by plain loads from here on: this kernel was running while the one before it wrote them, and the
+  // read-only path asks for memory that nobody writes during a kernel's whole life.
 
   if (warp == 0) {
     if (lane == 0) {
@@ -478,6 +480,11 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
   if (warp >= 2 && ok) {
     for (int c = 0; c < cols; c += 16) {
       uint32_t v[16];
+      float sx[16];                             // before the stores, which the compiler has to take for writes to them
+      if constexpr (S == 1) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sx[j] = c + j < cols ? p.sx[m0 + c + j] : 0.f;
+      }
       tmem_ld_32x16(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c, v);
       tmem_wait_ld();
 #pragma unroll
@@ -490,7 +497,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
                        : "=r"(addr) : "r"(smem_u32(part + (rank * (BM / S) + slot) * kI8BlockN + row)), "r"(owner));
           asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v[j]) : "memory");
         } else if (n < p.N) {
-          const float f = static_cast<float>(static_cast<int>(v[j])) * __ldg(p.sx + m0 + c + j) * swn;
+          const float f = static_cast<float>(static_cast<int>(v[j])) * sx[j] * swn;
           store_y<TY>(static_cast<TY*>(p.Y) + static_cast<long long>(m0 + c + j) * p.ldy + n, f);
         }
       }
@@ -505,7 +512,7 @@ gemm_int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
 #pragma unroll
         for (int r = 0; r < S; ++r) sum += part[(r * (BM / S) + slot) * kI8BlockN + row];
         const int m = m0 + slot * S + rank;
-        store_y<TY>(static_cast<TY*>(p.Y) + static_cast<long long>(m) * p.ldy + n, static_cast<float>(sum) * __ldg(p.sx + m) * swn);
+        store_y<TY>(static_cast<TY*>(p.Y) + static_cast<long long>(m) * p.ldy + n, static_cast<float>(sum) * p.sx[m] * swn);
       }
     }
   }

@@ -369,3 +369,32 @@ def test_values_are_the_nearest_to_the_quotient_by_the_stored_scale(M, K):
     q, s = ops.quantize_rows_int8(x)
     want, ws = quantize_rows_int8_reference(x.cpu())               # where / is a division
     assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 5, 40, 100, 700])
+def test_scales_written_by_the_kernel_before(M):
+    """The same memory holds other scales in every round; the product that reads them is set up while they are written."""
+    from steptronoss_b200 import ops
+
+    torch.manual_seed(6)
+    N, K, rounds = 1500, 768, 30
+    wq, sw = ops.quantize_rows_int8(torch.randn(N, K, device="cuda").to(torch.bfloat16))
+    xs = [(torch.randn(M, K, device="cuda") * 2.0 ** (r % 13 - 6)).to(torch.bfloat16) for r in range(rounds)]
+    want = []
+    for x in xs:
+        q, s = ops.quantize_rows_int8(x)
+        torch.cuda.synchronize()
+        want.append(ops.gemm_int8(q, s, wq, sw))
+        torch.cuda.synchronize()
+    for _ in range(3):
+        got = [ops.linear_int8(x, wq, sw) for x in xs]         # freed scales come back in the next round
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = torch.empty_like(xs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.linear_int8(x, wq, sw)
+    for src, ref in zip(xs, want):
+        x.copy_(src)
+        graph.replay()
+        assert torch.equal(y, ref)
