@@ -517,6 +517,12 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t phase) {
     if (mbar_try_wait(bar, phase)) return true;
   return mbar_wait(bar, phase);
 }
+// The cluster's pairs: with them the other CTAs say that they have read the logits that this one may overwrite.
+__device__ __forceinline__ bool mbar_wait_pairs(uint64_t* bar, uint32_t phase) {
+  for (int i = 0; i < 1024; ++i)
+    if (mbar_try_wait_cluster(bar, phase)) return true;
+  return mbar_wait_cluster(bar, phase);
+}
 __device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t phase, unsigned ns) {
   if (mbar_try_wait(bar, phase)) return true;
   const uint64_t t0 = global_timer_ns();
@@ -910,7 +916,7 @@ distill_row_kernel(const DistillParams p, const RowPlan plan) {
         if (threadIdx.x == 0) mbar_arrive_expect_tx(&bars.xchg[b], C * kRowWarps * 8);
         __syncwarp();
         if (lane < C) send_pair(&part[b][rank * kRowWarps + warp], &bars.xchg[b], lane, top, sum);
-        ok = ok && mbar_wait_soon(&bars.xchg[b], phase);
+        ok = ok && mbar_wait_pairs(&bars.xchg[b], phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) { leave(); break; }
         constexpr int kPairs = C * kRowWarps;

@@ -110,22 +110,6 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Bounded wait for an arrival that another CTA of the cluster may have made.
-__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 0; i < kSpinLimit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (ok) return true;
-    if (i == 0) t0 = global_timer_ns();
-    else if ((i & 255u) == 0 && global_timer_ns() - t0 > kWaitBudgetNs) return false;
-  }
-  return false;
-}
 // Whether `ok` holds for all 128 threads that meet at named barrier `id`.
 __device__ __forceinline__ bool group_and(int id, bool ok) {
   uint32_t r;
@@ -229,7 +213,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         int8_tile(tile, num_n, num_m, n_tile, m_tile);
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % kPairStages;
-          if (!mbar_wait_pair(&empty_bar[s], ((it / kPairStages) & 1) ^ 1)) {
+          if (!mbar_wait_cluster(&empty_bar[s], ((it / kPairStages) & 1) ^ 1)) {
             report_error(p.status, kErrProducerWait);
             *abort_flag = 1;
             break;
@@ -249,12 +233,12 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       bool ok = true;
       for (int tile = blockIdx.x / 2; tile < num_tiles && ok && !*abort_flag; tile += pairs, ++local) {
         const int acc = local & 1;
-        ok = mbar_wait_pair(&tmem_empty[acc], ((local >> 1) & 1) ^ 1);
+        ok = mbar_wait_cluster(&tmem_empty[acc], ((local >> 1) & 1) ^ 1);
         if (!ok) { report_error(p.status, kErrMmaWaitTmem); break; }
         tc_fence_after();
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % kPairStages;
-          ok = mbar_wait_pair(&full_bar[s], (it / kPairStages) & 1);
+          ok = mbar_wait_cluster(&full_bar[s], (it / kPairStages) & 1);
           if (!ok) { report_error(p.status, kErrMmaWaitFull); break; }
           tc_fence_after();
           const uint32_t sw = smem_u32(smem + s * kPairStageBytes);
@@ -281,7 +265,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const int n0 = cta_n0 + quarter * 32, n = n0 + lane, m0 = m_tile * kPairTile;
       const float sw = n < p.N ? p.sw[n] : 0.f;
       // the group goes on or leaves as one: its warps meet at barriers below
-      const bool ok = group_and(1 + group, mbar_wait_pair(&tmem_full[acc], (local >> 1) & 1));
+      const bool ok = group_and(1 + group, mbar_wait_cluster(&tmem_full[acc], (local >> 1) & 1));
       if (!ok) { report_error(p.status, kErrEpilogueWait); *abort_flag = 1; break; }
       tc_fence_after();
       const int cols = min(kPairTile, p.M - m0);

@@ -992,3 +992,23 @@ def test_fused_head_passes_over_hidden_states_that_do_not_count(device, main_gra
     live = torch.ones(T, dtype=torch.bool)
     live[dead] = False
     assert torch.equal(tok[live], want[1][live]) and tok[[3, 40, 69]].eq(0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,T,V,K", [(torch.bfloat16, 8, 151936, 1024), (torch.float32, 300, 151936, 200),
+                                         (torch.bfloat16, 700, 50257, 200)])
+def test_the_gradient_over_the_logits_waits_for_every_reader(dtype, T, V, K):
+    """The first CTA of a cluster reads the logits at all entries, wherever they lie, before others write over them."""
+    from steptronoss_b200.ops import topk_distillation_loss_and_grad
+
+    g = torch.Generator(device="cuda").manual_seed(24)
+    logits = (torch.randn(T, V, device="cuda", generator=g) * 3).to(dtype)
+    step = V // K
+    ids = torch.arange(K, device="cuda") * step + torch.randint(0, step, (T, K), device="cuda", generator=g)
+    teacher, w = torch.randn(T, K, device="cuda", generator=g), torch.rand(T, device="cuda", generator=g)
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    buf = torch.empty_like(logits)
+    for _ in range(20):
+        buf.copy_(logits)
+        again, _ = topk_distillation_loss_and_grad(buf, ids, teacher, w, out=buf)
+        assert torch.equal(again, loss) and torch.equal(buf, grad)
