@@ -624,7 +624,7 @@ extern "C" int stb_gemm_int8(const void* xq, const float* sx, const void* wq, co
                              int K, long long ldx, long long ldw, long long ldy, int out_f32, int* status,
                              cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || K > 131071 || (ldx & 15) || (ldw & 15) || ldx < K || ldw < K || ldy < N ||
+  if (M > (1 << 30) || N > (1 << 30) || K <= 0 || K > 131071 || (ldx & 15) || (ldw & 15) || ldx < K || ldw < K || ldy < N ||
       (reinterpret_cast<uintptr_t>(xq) & 15) || (reinterpret_cast<uintptr_t>(wq) & 15))
     return -kErrBadArgument;
   Int8GemmParams p{};

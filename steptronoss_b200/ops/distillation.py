@@ -29,6 +29,7 @@ from .cross_entropy import _all_reduce
 from .gemm import _tma_compatible, count_launch, gemm
 
 MAX_ENTRIES = 1024
+MAX_TOKENS, MAX_VOCAB = 0x0FFFFFFF, 1 << 30      # of a call; what the C entry points take, as 32-bit numbers
 P, I, L, F = native.P, native.I, native.L, native.F
 native.register_signature("stb_distill_row_limit", [I])
 native.register_signature("stb_distill_row", [P, L, P, L, P, I, L, P, L, P, P, P, I, I, I, F, I, I, P, P])
@@ -45,9 +46,11 @@ def _group_size(group) -> int:
     return dist.get_world_size(group) if group is not None else 1
 
 
-def _checked(rows: int, index: int, teacher_ids, teacher_logits, temperature, what: str):
+def _checked(rows: int, vocab: int, index: int, teacher_ids, teacher_logits, temperature, what: str):
     """Teacher entries as ``[rows, K]`` with a contiguous last dimension (ids int32 / int64, logits fp32); ``index`` is
     the student's device."""
+    if rows > MAX_TOKENS or vocab > MAX_VOCAB:
+        raise ValueError(f"{what}: {rows} tokens of {vocab} logits, at most {MAX_TOKENS} of {MAX_VOCAB} are taken")
     shape = teacher_ids.shape
     if shape != teacher_logits.shape or len(shape) < 1:
         raise ValueError(f"{what}: teacher_ids {tuple(shape)} and teacher_logits {tuple(teacher_logits.shape)} differ")
@@ -299,8 +302,9 @@ def topk_distillation(logits, teacher_ids, teacher_logits, temperature: float = 
     ``teacher_ids`` are always ids of the whole vocabulary.  Differentiable with respect to ``logits``."""
     temperature, vocab_start = float(temperature), int(vocab_start)
     rows = math.prod(logits.shape[:-1])
-    _check_shard(logits.shape[-1] if logits.dim() else 0, vocab_start, group, "topk_distillation")
-    ids, t = _checked(rows, logits.get_device(), teacher_ids, teacher_logits, temperature, "topk_distillation")
+    V = logits.shape[-1] if logits.dim() else 0
+    _check_shard(V, vocab_start, group, "topk_distillation")
+    ids, t = _checked(rows, V, logits.get_device(), teacher_ids, teacher_logits, temperature, "topk_distillation")
     return _TopkDistillationFn.apply(logits, ids, t, temperature, vocab_start, group)
 
 
@@ -324,7 +328,7 @@ def topk_distillation_loss_and_grad(logits, teacher_ids, teacher_logits, weights
     if logits.dim() != 2:
         raise ValueError(f"{what}: logits are [T, V], got {tuple(logits.shape)}")
     x, index = _rows_of(logits.detach() if logits.requires_grad else logits, what), logits.get_device()
-    ids, t = _checked(x.shape[0], index, teacher_ids, teacher_logits, temperature, what)
+    ids, t = _checked(x.shape[0], x.shape[1], index, teacher_ids, teacher_logits, temperature, what)
     w = _token_weights(weights, x.shape[0], index, what)
     if out is None:
         out = x.new_empty(x.shape)
@@ -471,7 +475,7 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
     _check_shard(w.shape[0], int(vocab_start), group, what)
     if w.device != h.device:
         raise ValueError(f"{what}: h on {h.device}, w on {w.device}")
-    ids, t = _checked(h.shape[0], h.get_device(), teacher_ids, teacher_logits, temperature, what)
+    ids, t = _checked(h.shape[0], w.shape[0], h.get_device(), teacher_ids, teacher_logits, temperature, what)
     wt = _token_weights(weights, h.shape[0], h.get_device(), what)
     if torch.is_grad_enabled():
         if weights.requires_grad:

@@ -18,6 +18,7 @@ from .gemm import count_launch
 
 INT8_MAX = 127.0
 MAX_K = 131071            # int32 sums of 128 * 128 stay below 2^31
+MAX_ROWS = 1 << 30        # tokens or channels of a product; its C entry point takes 32-bit numbers
 MAX_ROW = 32768           # widest row of the quantisation kernels
 P, I, L, F = native.P, native.I, native.L, native.F
 native.register_signature("stb_gemm_int8", [P, P, P, P, P, I, I, I, L, L, L, I, P, P])
@@ -67,6 +68,8 @@ def quantize_rows_int8(x: torch.Tensor):
         raise ValueError(f"quantize_rows_int8 takes [M, K], got {tuple(x.shape)}")
     _no_gradient("quantize_rows_int8", x)
     M, K = x.shape
+    if M > MAX_ROWS:
+        raise ValueError(f"quantize_rows_int8 takes at most {MAX_ROWS} rows, got {M}")
     if not x.is_cuda:
         q, s = quantize_rows_int8_reference(x)
         return pitched_like(q), s
@@ -122,6 +125,8 @@ def gemm_int8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
     if sx.dtype != torch.float32 or sw.dtype != torch.float32 or sx.shape != (M,) or sw.shape != (N,):
         raise ValueError(f"gemm_int8 takes fp32 scales [{M}] and [{N}], got {sx.dtype} {tuple(sx.shape)} and "
                          f"{sw.dtype} {tuple(sw.shape)}")
+    if M > MAX_ROWS or N > MAX_ROWS:
+        raise ValueError(f"gemm_int8 takes at most {MAX_ROWS} tokens and channels, got {M} and {N}")
     index = xq.get_device()              # -1 on the CPU
     if wq.get_device() != index or sx.get_device() != index or sw.get_device() != index:
         raise ValueError("gemm_int8: operands on different devices")

@@ -1012,3 +1012,25 @@ def test_the_gradient_over_the_logits_waits_for_every_reader(dtype, T, V, K):
         buf.copy_(logits)
         again, _ = topk_distillation_loss_and_grad(buf, ids, teacher, w, out=buf)
         assert torch.equal(again, loss) and torch.equal(buf, grad)
+
+
+@pytest.mark.parametrize("rows, vocab", [(2 ** 28, 1), (2 ** 31 + 1, 1), (2 ** 32 + 3, 1), (1, 2 ** 30 + 1), (1, 2 ** 32 + 3)])
+def test_sizes_beyond_the_kernels_are_refused(rows, vocab):
+    """Sizes cross the C interface as 32-bit numbers: larger ones would be taken for smaller ones there."""
+    from steptronoss_b200.ops import topk_distillation, topk_distillation_loss_and_grad
+
+    logits = torch.zeros(1, 1).expand(rows, vocab)
+    ids, teacher = torch.zeros(1, 1, dtype=torch.long).expand(rows, 1), torch.zeros(1, 1).expand(rows, 1)
+    with pytest.raises(ValueError, match="at most"):
+        topk_distillation(logits, ids, teacher)
+    with pytest.raises(ValueError, match="at most"):
+        topk_distillation_loss_and_grad(logits, ids, teacher, torch.zeros(1).expand(rows))
+
+
+def test_fused_head_refuses_sizes_beyond_the_kernels():
+    from steptronoss_b200.ops import fused_linear_topk_distillation as f
+
+    for rows, vocab in ((2 ** 31 + 8, 8), (1, 2 ** 32 + 8)):
+        ids, teacher = torch.zeros(1, 1, dtype=torch.long).expand(rows, 1), torch.zeros(1, 1).expand(rows, 1)
+        with pytest.raises(ValueError, match="at most"):
+            f(torch.zeros(1, 8).expand(rows, 8), torch.zeros(1, 8).expand(vocab, 8), ids, teacher, torch.zeros(1).expand(rows))

@@ -398,3 +398,16 @@ def test_scales_written_by_the_kernel_before(M):
         x.copy_(src)
         graph.replay()
         assert torch.equal(y, ref)
+
+
+@pytest.mark.parametrize("M, N", [(2 ** 30 + 1, 1), (1, 2 ** 31 + 1), (2 ** 32 + 3, 1)])
+def test_sizes_beyond_the_kernels_are_refused(M, N):
+    """Sizes cross the C interface as 32-bit numbers: larger ones would be taken for smaller ones there."""
+    from steptronoss_b200 import ops
+
+    row = lambda n: torch.zeros(1, 16, dtype=torch.int8).expand(n, 16)
+    scale = lambda n: torch.ones(1).expand(n)
+    with pytest.raises(ValueError, match="at most"):
+        ops.gemm_int8(row(M), scale(M), row(N), scale(N))
+    with pytest.raises(ValueError, match="at most"):
+        ops.linear_int8(torch.zeros(1, 16).expand(M, 16) if M > 1 else torch.zeros(1, 16), row(N), scale(N))
