@@ -241,11 +241,15 @@ __device__ __forceinline__ void warp_merge(float& m, float& s) {
   if (whole) s = -s;
 }
 
-// Teacher entries of a row in shared memory (statistics and gradient kernels).
+// Teacher entries of a chunk of a row in shared memory (gradient kernel).
 struct Entries {
   float q[kDsMaxEntries];      // probability, 0 where there is no entry
-  float s[kDsMaxEntries];      // the student's logit there (0 where the id is not in this shard)
-  int id[kDsMaxEntries];       // local id, -1 where there is no entry in this shard
+  float s[kDsMaxEntries];      // the student's logit there (0 where the id is not in this chunk)
+  int id[kDsMaxEntries];       // local id, -1 where there is no entry in this chunk
+};
+// Teacher statistics of a row (statistics kernel).
+struct TeacherRow {
+  float t[kDsMaxEntries];
   float tmax, tsum;            // tsum = 0: no entry at all
 };
 
@@ -260,8 +264,9 @@ __device__ __forceinline__ float entry_q(float t, float tmax, float inv_tsum, fl
   return ex2((t - tmax) * c) * inv_tsum;
 }
 
+// By one warp: the row's teacher statistics, and the student's logits at the ids that fall into this shard (0 at others).
 template <typename T>
-__device__ __forceinline__ void load_entries(const DistillParams& p, const T* row_ptr, long long row, Entries& e, int lane) {
+__device__ __forceinline__ void load_teacher(const DistillParams& p, const T* row_ptr, long long row, TeacherRow& e, int lane) {
   const float c = p.inv_tau * kLog2e;
   float tmax = -INFINITY;
   bool bad = false;            // fmaxf drops a NaN; it has to reach the loss
@@ -271,9 +276,8 @@ __device__ __forceinline__ void load_entries(const DistillParams& p, const T* ro
     const float t = in ? p.teacher[row * p.ld_t + j] : -INFINITY;
     const long long local = id - p.vocab_start;
     const bool here = in && t != -INFINITY && local >= 0 && local < p.V;
-    e.q[j] = t;
-    e.id[j] = here ? static_cast<int>(local) : -1;
-    e.s[j] = here ? Lane<T>::value(row_ptr + local) : 0.f;
+    e.t[j] = t;
+    p.picked[row * p.K + j] = here ? Lane<T>::value(row_ptr + local) : 0.f;
     tmax = fmaxf(tmax, t);
     bad |= t != t;
   }
@@ -282,12 +286,10 @@ __device__ __forceinline__ void load_entries(const DistillParams& p, const T* ro
   if (__any_sync(0xffffffffu, bad)) tmax = __uint_as_float(0x7FC00000u);
   float tsum = 0.f;
   if (tmax != -INFINITY) {
-    for (int j = lane; j < p.K; j += 32) tsum += ex2((e.q[j] - tmax) * c);
+    for (int j = lane; j < p.K; j += 32) tsum += ex2((e.t[j] - tmax) * c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) tsum += __shfl_xor_sync(0xffffffffu, tsum, o);
   }
-  const float inv = tmax != -INFINITY ? __fdiv_rn(1.f, tsum) : 0.f;
-  for (int j = lane; j < p.K; j += 32) e.q[j] = tmax != -INFINITY ? entry_q(e.q[j], tmax, inv, c) : 0.f;
   if (lane == 0) { e.tmax = tmax; e.tsum = tsum; }
 }
 
@@ -1012,17 +1014,14 @@ template <typename T>
 __global__ void __launch_bounds__(kDsStatsThreads)
 distill_stats_kernel(const DistillParams p) {
   constexpr int n = Lane<T>::n;
-  __shared__ Entries e;
+  __shared__ TeacherRow e;
   __shared__ float2 red[kDsStatsThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long row = blockIdx.x;
   const T* src = static_cast<const T*>(p.logits) + row * p.ld;
   const Granules<T> gr(src, p.V);
   const float c = p.inv_tau * kLog2e;
-  if (warp == 0) {
-    load_entries<T>(p, src, row, e, lane);
-    for (int j = lane; j < p.K; j += 32) p.picked[row * p.K + j] = e.s[j];
-  }
+  if (warp == 0) load_teacher<T>(p, src, row, e, lane);
   float top = -INFINITY, sum = 0.f;
   constexpr int kUnroll = 4;
   for (int g0 = threadIdx.x; g0 < gr.count; g0 += kDsStatsThreads * kUnroll) {
