@@ -71,28 +71,6 @@ __device__ __forceinline__ bool usable(float amax) { return amax >= 6e-36f && am
 __device__ __forceinline__ float scale_of(float amax, float steps) {
   return usable(amax) ? __fdiv_rn(amax, steps) : amax < 6e-36f ? 1.f : __uint_as_float(0x7FC00000u);
 }
-// Two fp32 at once: one instruction on this architecture.
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // y / scale, rounded once: the quotient by the rounded reciprocal, corrected by its remainder (Markstein, IBM J. Res. Dev.
 // 34(1), 1990), so that the 8-bit value is the one that a division by the stored scale gives.  A product with the
 // reciprocal alone misses neighbours of a border between two values, and bf16 rows hold many of them (63.5 steps at half of
@@ -103,10 +81,10 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 struct Divisor {
   uint64_t minus_scale, inverse;                   // 0, 0: everything finite becomes 0
   __device__ __forceinline__ Divisor(float amax, float scale)
-      : minus_scale(usable(amax) ? pack2(-scale, -scale) : 0), inverse(0) {
+      : minus_scale(usable(amax) ? pair(-scale, -scale) : 0), inverse(0) {
     if (usable(amax)) {
       const float r = __frcp_rn(scale);
-      inverse = pack2(r, r);
+      inverse = pair(r, r);
     }
   }
   __device__ __forceinline__ uint64_t divide(uint64_t y) const {
@@ -120,10 +98,10 @@ struct Divisor {
   }
 };
 __device__ __forceinline__ void widen4x2(const uint4& u, uint64_t (&f)[4]) {
-  f[0] = pack2(bf16_lo(u.x), bf16_hi(u.x));
-  f[1] = pack2(bf16_lo(u.y), bf16_hi(u.y));
-  f[2] = pack2(bf16_lo(u.z), bf16_hi(u.z));
-  f[3] = pack2(bf16_lo(u.w), bf16_hi(u.w));
+  f[0] = pair(bf16_lo(u.x), bf16_hi(u.x));
+  f[1] = pair(bf16_lo(u.y), bf16_hi(u.y));
+  f[2] = pair(bf16_lo(u.z), bf16_hi(u.z));
+  f[3] = pair(bf16_lo(u.w), bf16_hi(u.w));
 }
 // bf16(a + b) of two pairs.  One rounding of the exact sum is what an fp32 addition followed by a rounding gives: the fp32
 // sum of two bf16 numbers is inexact only where one of them is too small to move the other at all.
@@ -246,7 +224,7 @@ norm_quant_kernel(const NormQuantParams p) {
       for (int j = 0; j < 4; ++j) ss2 = fma2(f[j], f[j], ss2);
     }
     float a, b;
-    unpack2(ss2, a, b);
+    unpair(ss2, a, b);
     rstd = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(a + b, red_sum), static_cast<float>(p.H)) + p.eps);
   }
 
@@ -258,17 +236,17 @@ norm_quant_kernel(const NormQuantParams p) {
     widen4x2(load8<A, TPR>(p.w, tid, i, p.H), g);
     if (p.zero_centered) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = add2(g[j], pack2(1.f, 1.f));
+      for (int j = 0; j < 4; ++j) g[j] = add2(g[j], pair(1.f, 1.f));
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = mul2(mul2(f[j], pack2(rstd, rstd)), g[j]);
+    for (int j = 0; j < 4; ++j) f[j] = mul2(mul2(f[j], pair(rstd, rstd)), g[j]);
   };
   auto top_of = [](const uint64_t (&f)[4]) {
     float m = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float a, b;
-      unpack2(f[j], a, b);
+      unpair(f[j], a, b);
       m = max_nan(m, max_nan(fabsf(a), fabsf(b)));
     }
     return m;
@@ -292,8 +270,8 @@ norm_quant_kernel(const NormQuantParams p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float a, b, c, d;
-        unpack2(by.divide(f[2 * h]), a, b);
-        unpack2(by.divide(f[2 * h + 1]), c, d);
+        unpair(by.divide(f[2 * h]), a, b);
+        unpair(by.divide(f[2 * h + 1]), c, d);
         const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
         out[h] = lo | (hi << 16);
@@ -329,7 +307,7 @@ norm_quant_kernel(const NormQuantParams p) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float a, b;
-            unpack2(add2(by.divide(f[2 * h + j]), pack2(12582912.f, 12582912.f)), a, b);
+            unpair(add2(by.divide(f[2 * h + j]), pair(12582912.f, 12582912.f)), a, b);
             r[2 * j] = __float_as_uint(a);
             r[2 * j + 1] = __float_as_uint(b);
           }
