@@ -68,24 +68,34 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 // Whether max|y| gives a scale.  Below 6e-36 max / 448 leaves the range of normal numbers; such values count as zero.
 __device__ __forceinline__ bool usable(float amax) { return amax >= 6e-36f && amax < INFINITY; }
-__device__ __forceinline__ float scale_of(float amax, float steps) {
-  return usable(amax) ? __fdiv_rn(amax, steps) : amax < 6e-36f ? 1.f : __uint_as_float(0x7FC00000u);
+__device__ __forceinline__ float scale_of(float amax, float quotient) {
+  return usable(amax) ? quotient : amax < 6e-36f ? 1.f : __uint_as_float(0x7FC00000u);
 }
-// y / scale, rounded once: the quotient by the rounded reciprocal, corrected by its remainder (Markstein, IBM J. Res. Dev.
-// 34(1), 1990), so that the 8-bit value is the one that a division by the stored scale gives.  A product with the
-// reciprocal alone misses neighbours of a border between two values, and bf16 rows hold many of them (63.5 steps at half of
-// a largest value that is a power of two).  Without .ftz: the remainder of a small y is not a normal number.  8 of about 100
-// instructions per eight columns: 16384 x 4096 to e4m3 70.2 us with either.  Plain int8 rows of that size take 37.4 us
-// instead of 34.7 (36 registers instead of 32 leave six CTAs on an SM; held to 32 they take 35.1, but the norms, which
-// spill then, 70.9).
+// x / 448 by its reciprocal in two parts, off by 2^-48 before the rounding.  A seventh has a distance of a fourteenth of a
+// unit in the last place at least from where the rounding turns: this is the rounded quotient.
+__device__ __forceinline__ float over_448(float x) {
+  constexpr float hi = static_cast<float>(1.0 / 448), lo = static_cast<float>(1.0 / 448 - static_cast<double>(hi));
+  return fmaf(x, hi, x * lo);
+}
+// y / d, rounded once: the quotient by the rounded reciprocal, corrected by its remainder (Markstein, IBM J. Res. Dev. 34(1),
+// 1990).  A product with the reciprocal alone misses neighbours of a border between two 8-bit values, and bf16 rows hold
+// many quotients that lie on one (63.5 steps at half of a largest value that is a power of two).  Without .ftz: the
+// remainder of a small y is not a normal number.  8 of about 100 instructions per eight columns: 16384 x 4096 to e4m3 70.3 us
+// instead of 70.0 us.  Plain int8 rows of that size take 37.4 us instead of 34.7 (36 registers instead of 32 leave six
+// CTAs on an SM; held to 32 they take 35.1, but the norms, which spill then, 70.9).
+//
+// int8 divides by the stored scale.  e4m3 divides two exact numbers: rsqrt is the same factor in y and max|y|, so that only
+// its power of two is kept there (7/8 of it, since 448 is 7/8 of 2^9); s * w is a product of two bf16 numbers, t = 7/8 s w
+// has 19 bits, and 448 y / max|y| is t over a 448-th of the largest t.  It lies on a border between two values exactly
+// where it does in real numbers, and takes the even one.  (The weight 1 + w of a zero-centred norm has more bits: one
+// rounding.)
 struct Divisor {
-  uint64_t minus_scale, inverse;                   // 0, 0: everything finite becomes 0
-  __device__ __forceinline__ Divisor(float amax, float scale)
-      : minus_scale(usable(amax) ? pair(-scale, -scale) : 0), inverse(0) {
-    if (usable(amax)) {
-      const float r = __frcp_rn(scale);
-      inverse = pair(r, r);
-    }
+  uint64_t minus_by, inverse;                      // 0, 0: everything finite becomes 0
+  __device__ __forceinline__ Divisor(bool some, float by) : minus_by(0), inverse(0) {
+    if (!some) return;
+    const float r = __frcp_rn(by);
+    minus_by = pair(-by, -by);
+    inverse = pair(r, r);
   }
   __device__ __forceinline__ uint64_t divide(uint64_t y) const {
     uint64_t q;
@@ -93,7 +103,7 @@ struct Divisor {
         "mul.rn.f32x2 q, %1, %3;\n\t"
         "fma.rn.f32x2 e, q, %2, %1;\n\t"
         "fma.rn.f32x2 %0, e, %3, q;\n\t}"
-        : "=l"(q) : "l"(y), "l"(minus_scale), "l"(inverse));
+        : "=l"(q) : "l"(y), "l"(minus_by), "l"(inverse));
     return q;
   }
 };
@@ -228,6 +238,10 @@ norm_quant_kernel(const NormQuantParams p) {
     rstd = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(a + b, red_sum), static_cast<float>(p.H)) + p.eps);
   }
 
+  // e4m3: the power of two of rsqrt goes into y, its mantissa into the scales (1 where there is none: 0, infinity)
+  const float factor = E4M3 ? 0.875f * __uint_as_float(__float_as_uint(rstd) & 0x7F800000u) : rstd;
+  const float mantissa = __uint_as_float((__float_as_uint(rstd) & 0x007FFFFFu) | 0x3F800000u);
+
   // y of eight columns, in fp32 (recomputed where it is needed twice and not kept: the registers hold the bf16 sum)
   auto normed = [&](int i, uint64_t (&f)[4]) {
     widen4x2(v[i], f);
@@ -239,7 +253,7 @@ norm_quant_kernel(const NormQuantParams p) {
       for (int j = 0; j < 4; ++j) g[j] = add2(g[j], pair(1.f, 1.f));
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = mul2(mul2(f[j], pair(rstd, rstd)), g[j]);
+    for (int j = 0; j < 4; ++j) f[j] = mul2(mul2(f[j], pair(factor, factor)), g[j]);
   };
   auto top_of = [](const uint64_t (&f)[4]) {
     float m = 0.f;
@@ -264,8 +278,8 @@ norm_quant_kernel(const NormQuantParams p) {
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (k * 8 >= p.H) continue;
-      const float scale = scale_of(m, 448.f);
-      const Divisor by(m, scale);
+      const float top = over_448(m), amax = top * 512.f * mantissa;
+      const Divisor by(usable(amax), top);
       uint32_t out[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -277,7 +291,7 @@ norm_quant_kernel(const NormQuantParams p) {
         out[h] = lo | (hi << 16);
       }
       store8_bytes<A, TPR>(qr, tid, i, p.H, out[0], out[1]);
-      if ((k & 15) == 0) p.scale[row * kbs + (k >> 4)] = scale;
+      if ((k & 15) == 0) p.scale[row * kbs + (k >> 4)] = scale_of(amax, over_448(amax));
     }
   } else {
     constexpr bool kKeep = NV <= 2;            // y stays in registers where it is small
@@ -290,8 +304,8 @@ norm_quant_kernel(const NormQuantParams p) {
       m = max_nan(m, top_of(f));
     }
     m = row_max<TPR>(m, red_max);
-    const float scale = scale_of(m, 127.f);
-    const Divisor by(m, scale);
+    const float scale = scale_of(m, __fdiv_rn(m, 127.f));
+    const Divisor by(usable(m), scale);
     if (tid == 0) p.scale[row] = scale;
     const bool some = usable(m);
 #pragma unroll

@@ -229,7 +229,6 @@ def test_rows_up_to_the_largest_number(device, fmt):
 def test_values_behind_the_norm_are_the_nearest_to_the_quotient(T, H):
     """With |s| = 1 throughout and eps = 0 the norm is exact: y = +-w."""
     from steptronoss_b200 import ops
-    from steptronoss_b200.ops.norm_quant import _quantized_e4m3
     from steptronoss_b200.ops.int8 import quantize_rows_int8_reference
 
     torch.manual_seed(5)
@@ -241,5 +240,27 @@ def test_values_behind_the_norm_are_the_nearest_to_the_quotient(T, H):
     want, ws = quantize_rows_int8_reference(y)
     assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), want)
     q, s = ops.rmsnorm_quant(x, w, 0.0, fmt="e4m3_1x128")
-    want, ws = _quantized_e4m3(y)
-    assert torch.equal(s.cpu(), ws) and torch.equal(q.float().cpu(), want.float())
+    b = y.view(T, H // 128, 128)
+    top = b.abs().amax(2, keepdim=True)
+    want = (448 * b.double() / top.double()).float().to(torch.float8_e4m3fn).view(T, H)
+    assert torch.equal(s.cpu(), (top / 448).squeeze(2)) and torch.equal(q.float().cpu(), want.float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", [(64, 512), (4, 4096), (300, 4096), (100, 1280), (3, 32768)])
+def test_e4m3_values_are_those_of_the_definition(T, H):
+    """448 y / max|y| in real numbers: the norm's factor drops out, and 448 s w has 19 bits.  In 64 bits the quotient is off
+    by 2^-51 of itself; one that lies on a border between two e4m3 values is put back there by the rounding to fp32, which
+    any other is too far from (the numerator and the border times max|y| are integers of less than 30 bits)."""
+    from steptronoss_b200 import ops
+
+    x, d, w = make(T, H, "cuda")
+    x[0, :128], d[0, :128] = x[0, :128].abs().log2().round().exp2(), 0              # powers of two
+    s, y = exact(x, d, w, 1e-6)
+    b = y.view(T, H // 128, 128)
+    want = (448 * b / b.abs().amax(2, keepdim=True)).float().to(torch.float8_e4m3fn).view(T, H)
+    _, q, sc = ops.add_rmsnorm_quant(x, d, w, 1e-6, fmt="e4m3_1x128")
+    assert torch.equal(q.float(), want.float())
+    check_e4m3(q, sc, y)
+    q, _ = ops.rmsnorm_quant(s, w, 1e-6, fmt="e4m3_1x128")
+    assert torch.equal(q.float(), want.float())
