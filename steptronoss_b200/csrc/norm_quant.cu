@@ -77,12 +77,12 @@ __device__ __forceinline__ float over_448(float x) {
   constexpr float hi = static_cast<float>(1.0 / 448), lo = static_cast<float>(1.0 / 448 - static_cast<double>(hi));
   return fmaf(x, hi, x * lo);
 }
-// y / d, rounded once: the quotient by the rounded reciprocal, corrected by its remainder (Markstein, IBM J. Res. Dev. 34(1),
-// 1990).  A product with the reciprocal alone misses neighbours of a border between two 8-bit values, and bf16 rows hold
-// many quotients that lie on one (63.5 steps at half of a largest value that is a power of two).  Without .ftz: the
-// remainder of a small y is not a normal number.  8 of about 100 instructions per eight columns: 16384 x 4096 to e4m3 70.3 us
-// instead of 70.0 us.  Plain int8 rows of that size take 37.4 us instead of 34.7 (36 registers instead of 32 leave six
-// CTAs on an SM; held to 32 they take 35.1, but the norms, which spill then, 70.9).
+// y / d, rounded once: the reciprocal in two parts, its rounded value and what that leaves, so that the quotient is off by
+// 2^-46 of itself before its rounding (while d is below 2^100 and the second part a normal number).  The rounded reciprocal
+// alone misses neighbours of a border between two 8-bit values, and bf16 rows hold many quotients that lie on one (63.5 steps
+// at half of a largest value that is a power of two).  4 of about 100 instructions per eight columns, and registers that have
+// to be held at 32 for whole occupancy: 16384 x 4096 to int8 71.1 us (70.3 with the reciprocal alone), to e4m3 72.1 (71.6),
+// plain int8 rows 33.9 (34.1).
 //
 // int8 divides by the stored scale.  e4m3 divides two exact numbers: rsqrt is the same factor in y and max|y|, so that only
 // its power of two is kept there (7/8 of it, since 448 is 7/8 of 2^9); s * w is a product of two bf16 numbers, t = 7/8 s w
@@ -90,20 +90,19 @@ __device__ __forceinline__ float over_448(float x) {
 // where it does in real numbers, and takes the even one.  (The weight 1 + w of a zero-centred norm has more bits: one
 // rounding.)
 struct Divisor {
-  uint64_t minus_by, inverse;                      // 0, 0: everything finite becomes 0
-  __device__ __forceinline__ Divisor(bool some, float by) : minus_by(0), inverse(0) {
+  uint64_t high, low;                              // 1 / d in two parts; 0, 0: everything finite becomes 0
+  __device__ __forceinline__ Divisor(bool some, float d) : high(0), low(0) {
     if (!some) return;
-    const float r = __frcp_rn(by);
-    minus_by = pair(-by, -by);
-    inverse = pair(r, r);
+    const float r = __frcp_rn(d), rest = fmaf(-d, r, 1.f) * r;
+    high = pair(r, r);
+    low = pair(rest, rest);
   }
   __device__ __forceinline__ uint64_t divide(uint64_t y) const {
     uint64_t q;
-    asm("{\n\t.reg .b64 q, e;\n\t"
-        "mul.rn.f32x2 q, %1, %3;\n\t"
-        "fma.rn.f32x2 e, q, %2, %1;\n\t"
-        "fma.rn.f32x2 %0, e, %3, q;\n\t}"
-        : "=l"(q) : "l"(y), "l"(minus_by), "l"(inverse));
+    asm("{\n\t.reg .b64 t;\n\t"
+        "mul.rn.f32x2 t, %1, %3;\n\t"
+        "fma.rn.f32x2 %0, %1, %2, t;\n\t}"
+        : "=l"(q) : "l"(y), "l"(high), "l"(low));
     return q;
   }
 };
@@ -133,6 +132,10 @@ template <Access A, int TPR>
 __device__ __forceinline__ int column(int tid, int i, int j) {     // of pair j
   return A == kVec || A == kBlock ? 8 * (tid + i * TPR) + 2 * j : 2 * (tid + (4 * i + j) * TPR);
 }
+// Whether the warp of this thread has columns in round i at all (16384 x 5120: 102 us, 109 when all warps go through both
+// rounds).
+template <Access A, int TPR>
+__device__ __forceinline__ bool warp_has(int tid, int i, int H) { return column<A, TPR>(tid & ~31, i, 0) < H; }
 // Columns from H on read as zero.
 template <Access A, int TPR>
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int tid, int i, int H) {
@@ -193,7 +196,7 @@ __device__ __forceinline__ void store8_bytes(uint8_t* row, int tid, int i, int H
 
 // TPR threads share a row (a whole CTA, or one of the CTA's four warps when TPR is 32); NV times 8 columns per thread.
 template <int TPR, int NV, bool E4M3, Access A>
-__global__ void __launch_bounds__(TPR < 128 ? (TPR == 32 ? 128 : TPR) : TPR)
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, NV <= 2 && A == kVec ? 2048 / (TPR == 32 ? 128 : TPR) : 1)
 norm_quant_kernel(const NormQuantParams p) {
   __shared__ float red_sum[32];
   __shared__ uint32_t red_max[32];
@@ -271,6 +274,7 @@ norm_quant_kernel(const NormQuantParams p) {
     const int kbs = p.H / 128;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (i > 0 && !warp_has<A, TPR>(tid, i, p.H)) break;
       const int k = tid + i * TPR;
       uint64_t f[4];
       normed(i, f);
@@ -310,6 +314,7 @@ norm_quant_kernel(const NormQuantParams p) {
     const bool some = usable(m);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (i > 0 && !warp_has<A, TPR>(tid, i, p.H)) break;
       uint64_t (&f)[4] = y[kKeep ? i : 0];
       if constexpr (!kKeep) normed(i, f);
       uint32_t out[2] = {0u, 0u};
