@@ -1034,3 +1034,21 @@ def test_fused_head_refuses_sizes_beyond_the_kernels():
         ids, teacher = torch.zeros(1, 1, dtype=torch.long).expand(rows, 1), torch.zeros(1, 1).expand(rows, 1)
         with pytest.raises(ValueError, match="at most"):
             f(torch.zeros(1, 8).expand(rows, 8), torch.zeros(1, 8).expand(vocab, 8), ids, teacher, torch.zeros(1).expand(rows))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V", [(6, 151936), (300, 50257)])
+def test_large_rows_are_looked_at_again_before_they_are_overwritten(dtype, T, V):
+    from steptronoss_b200.ops import native, topk_distillation_loss_and_grad
+
+    (logits, ids, teacher, w), verify = lowest_rows(T, V, 9, dtype, "cuda", 1.0)
+    loss, grad = topk_distillation_loss_and_grad(logits, ids, teacher, w)
+    verify(loss, grad)
+    buf = torch.empty_like(logits)
+    for _ in range(10):
+        buf.copy_(logits)
+        again, _ = topk_distillation_loss_and_grad(buf, ids, teacher, w, out=buf)
+        assert torch.equal(again, loss) and torch.equal(buf, grad)
+    torch.cuda.synchronize()
+    native.raise_if_kernel_error()
