@@ -54,6 +54,8 @@ struct DistillParams {
   int* status;                  // row kernel: error word of its bounded waits
 };
 
+// 2 units in the last place, results below 2^-126 as 0: p is off by 1e-7 of itself, and what is flushed lies 2^-126 below a
+// row's largest probability.  Tenfold instructions for the last bit would make bf16 rows wait for arithmetic.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -380,7 +382,7 @@ constexpr int kMaxChunks = 12;
 struct RowPlan {
   int per;             // granules per CTA
   int chunks;          // per slice
-  int ring;            // chunks in shared memory, at least those of a slice where both passes are made
+  int ring;            // chunks in shared memory: two at least, and often fewer than a slice has
   int keep;            // last chunks of a slice that stay in the ring between the two passes; the others are loaded again
   int kpad;            // K rounded up to 4
 };
