@@ -1052,3 +1052,48 @@ def test_large_rows_are_looked_at_again_before_they_are_overwritten(dtype, T, V)
         assert torch.equal(again, loss) and torch.equal(buf, grad)
     torch.cuda.synchronize()
     native.raise_if_kernel_error()
+
+
+def _join_worker(rank, world, port, q):
+    os.environ.update(RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank), MASTER_ADDR="127.0.0.1",
+                      MASTER_PORT=str(port))
+    torch.set_num_threads(1)
+    try:
+        import torch.distributed as dist
+
+        from steptronoss_b200.ops.distillation import _join_shards
+
+        dist.init_process_group("gloo", rank=rank, world_size=world)
+        shard = [[(5.0, 2.0), (-3.4e38, -7.0), (-3.4e38, -7.0), (-INF, 0.0)],
+                 [(3.0, 4.0), (3.0, 4.0), (-3.4e38, -2.0), (9.0, 1.5)]][rank]
+        stats = torch.tensor([(*pair, 1.0, 2.0) for pair in shard])
+        picked = torch.full((4, 3), float(rank))
+        _join_shards(stats, picked, dist.group.WORLD)
+        q.put((rank, stats.tolist(), picked.tolist(), None))
+        dist.barrier()
+        dist.destroy_process_group()
+    except BaseException:
+        import traceback
+
+        q.put((rank, None, None, traceback.format_exc()))
+        raise
+
+
+def test_shards_are_joined_over_a_group():
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = free_port()
+    procs = [ctx.Process(target=_join_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    try:
+        for _ in range(2):
+            _, stats, picked, err = q.get(timeout=120)
+            assert err is None, err
+            want = torch.tensor([(5.0, 3.0, 1.0, 2.0), (3.0, 4.0, 1.0, 2.0), (-3.4e38, -9.0, 1.0, 2.0), (9.0, 1.5, 1.0, 2.0)])
+            assert torch.equal(torch.tensor(stats), want) and torch.tensor(picked).eq(1).all()
+    finally:
+        for p in procs:
+            p.join(timeout=30)
+            if p.is_alive():
+                p.kill()
