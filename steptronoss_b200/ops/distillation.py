@@ -476,6 +476,13 @@ def fused_linear_topk_distillation(h, w, teacher_ids, teacher_logits, weights, t
     temperature = float(temperature)
     if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1]:
         raise ValueError(f"{what}: h is [T, H] and w [V, H], got {tuple(h.shape)} and {tuple(w.shape)}")
+    if not w.numel():
+        raise ValueError(f"{what}: w needs a vocabulary and a hidden size, got {tuple(w.shape)}")
+    main_grad = getattr(w, "main_grad", None)
+    if main_grad is not None and (main_grad.shape != w.shape or main_grad.device != w.device
+                                  or main_grad.dtype not in (torch.float32, torch.bfloat16)):
+        raise ValueError(f"{what}: main_grad is fp32 or bf16 and lies beside w {tuple(w.shape)}, got {main_grad.dtype} "
+                         f"{tuple(main_grad.shape)} on {main_grad.device}")
     if chunk_tokens < 1:
         raise ValueError(f"{what}: chunk_tokens must be positive, got {chunk_tokens}")
     _check_shard(w.shape[0], int(vocab_start), group, what)

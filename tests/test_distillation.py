@@ -1097,3 +1097,23 @@ def test_shards_are_joined_over_a_group():
             p.join(timeout=30)
             if p.is_alive():
                 p.kill()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_fused_head_refuses_a_main_grad_that_does_not_fit(device):
+    """The weight gradient's product goes by the shape of w: it would write behind a smaller main_grad."""
+    from steptronoss_b200.ops import fused_linear_topk_distillation as f
+
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    ids, t, w = torch.zeros(4, 2, dtype=torch.long, device=device), torch.zeros(4, 2, device=device), torch.ones(4, device=device)
+    h, head = torch.zeros(4, 8, device=device, dtype=dtype), torch.nn.Parameter(torch.zeros(16, 8, device=device, dtype=dtype))
+    for bad in (torch.zeros(8, 8, device=device), torch.zeros(128, device=device), torch.zeros(16, 16, device=device),
+                torch.zeros(16, 8, device=device, dtype=torch.float16), torch.zeros(16, 8, device="meta")):
+        head.main_grad = bad
+        with pytest.raises(ValueError, match="main_grad"):
+            f(h, head, ids, t, w)
+    head.main_grad = torch.zeros(16, 8, device=device)
+    f(h, head, ids, t, w)
+    for empty in (torch.zeros(0, 8, device=device, dtype=dtype), torch.zeros(16, 0, device=device, dtype=dtype)):
+        with pytest.raises(ValueError, match="vocabulary"):
+            f(h[:, :empty.shape[1]], empty, ids, t, w)
